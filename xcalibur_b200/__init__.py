@@ -5,7 +5,8 @@ hand-written CUDA behind a C-ABI library (``include/xcb_moe.h``), driven from Py
 """
 from . import gf2, packer  # noqa: F401  (pure-Python layout machinery)
 
-__all__ = ["gf2", "packer", "moe_w4a16", "prepare", "kernel_fn", "PreparedMoE"]
+__all__ = ["gf2", "packer", "moe_w4a16", "prepare", "kernel_fn", "PreparedMoE", "PagedKVCache", "Rope",
+           "qk_norm_rope"]
 
 
 def __getattr__(name):
@@ -14,4 +15,8 @@ def __getattr__(name):
         from . import moe
 
         return getattr(moe, name)
+    if name in ("PagedKVCache", "Rope", "qk_norm_rope"):
+        from . import kvcache
+
+        return getattr(kvcache, name)
     raise AttributeError(name)

@@ -30,6 +30,13 @@ XCB_FLAG_PREFILL_PATH = 4
 XCB_FLAG_PDL = 8
 XCB_FLAG_DETERMINISTIC = 16
 XCB_STATIC_SCRATCH_BYTES = 8 << 20
+XCB_DTYPE_BF16 = 0
+XCB_DTYPE_F16 = 1
+XCB_DTYPE_E4M3 = 2
+XCB_DTYPE_F32 = 3
+XCB_STATUS_BAD_PAGE = 16
+XCB_STATUS_BAD_SEQ = 32
+XCB_STATUS_NO_PAGES = 64
 
 # every symbol include/xcb_moe.h declares
 EXPORTS = (
@@ -62,6 +69,22 @@ EXPORTS = (
     "xcb_ep_combine",
 )
 
+# every symbol include/xcb_attn.h declares
+ATTN_EXPORTS = (
+    "xcb_qk_norm_rope",
+    "xcb_attn_workspace_bytes",
+    "xcb_attn_workspace_init",
+    "xcb_paged_attention",
+    "xcb_kv_workspace_bytes",
+    "xcb_kv_workspace_init",
+    "xcb_kv_extend",
+    "xcb_kv_fork",
+    "xcb_kv_truncate",
+    "xcb_kv_compact",
+    "xcb_kv_copy_pages",
+    "xcb_kv_read_status",
+)
+
 
 class XcbMoeShape(ctypes.Structure):
     _fields_ = [("num_experts", ctypes.c_int32), ("total_experts", ctypes.c_int32), ("expert_offset", ctypes.c_int32),
@@ -78,6 +101,30 @@ class XcbMoeArgs(ctypes.Structure):
                 ("wait_limit_us", ctypes.c_int32), ("hidden_states", ctypes.c_void_p), ("router_logits", ctypes.c_void_p),
                 ("topk_ids", ctypes.c_void_p), ("topk_weights", ctypes.c_void_p), ("out", ctypes.c_void_p),
                 ("topk_ids_out", ctypes.c_void_p), ("topk_weights_out", ctypes.c_void_p)]
+
+
+class XcbKvCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("layers", "num_pages", "kv_heads", "page_size", "head_dim", "dtype",
+                                               "max_seqs", "max_pages")] + \
+               [(n, ctypes.c_void_p) for n in ("kv", "page_table", "seq_lens", "refcounts", "k_scale", "v_scale",
+                                                "status")]
+
+
+class XcbRopeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "q_heads", "kv_heads", "head_dim", "rotary_dim",
+                                               "interleaved", "dtype", "weight_dtype")] + \
+               [(n, ctypes.c_float) for n in ("eps", "weight_offset", "mscale")] + [("layer", ctypes.c_int32)] + \
+               [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride",
+                                                   "k_out_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("q_out", "k_out", "q_weight", "k_weight", "positions", "seqs",
+                                                "turns")]
+
+
+class XcbAttnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "new_tokens", "q_heads", "dtype", "layer", "window")] + \
+               [("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3),
+                ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("seqs", ctypes.c_void_p)]
 
 
 _LIB = None
@@ -123,6 +170,19 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "xcb_ep_p2p_combine": (ctypes.c_int, [P, I32, I32, I32, I32, I32, I32, P, P, P, U64, P]),
         "xcb_ep_gather": (ctypes.c_int, [P, P, P, I32, I32, I32, I32, P, P, P, P, P, P]),
         "xcb_ep_combine": (ctypes.c_int, [P, P, P, I32, I32, I32, P, P]),
+        # struct pointers as plain pointers: their owners keep the addresses, which makes a call cheaper
+        "xcb_qk_norm_rope": (ctypes.c_int, [P, P, P]),
+        "xcb_attn_workspace_bytes": (SZ, [P, I32, I32]),
+        "xcb_attn_workspace_init": (ctypes.c_int, [P, SZ, P]),
+        "xcb_paged_attention": (ctypes.c_int, [P, P, P, SZ, P]),
+        "xcb_kv_workspace_bytes": (SZ, [P]),
+        "xcb_kv_workspace_init": (ctypes.c_int, [P, P, SZ, P]),
+        "xcb_kv_extend": (ctypes.c_int, [P, P, P, I32, P, SZ, P]),
+        "xcb_kv_fork": (ctypes.c_int, [P, P, P, I32, P]),
+        "xcb_kv_truncate": (ctypes.c_int, [P, P, P, I32, P]),
+        "xcb_kv_compact": (ctypes.c_int, [P, P, SZ, P]),
+        "xcb_kv_copy_pages": (ctypes.c_int, [P, P, P, I32, P]),
+        "xcb_kv_read_status": (ctypes.c_int, [P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

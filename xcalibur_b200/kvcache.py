@@ -1,0 +1,435 @@
+"""The attention side of a decoder layer: a paged key-value cache and the operators on it.
+
+``PagedKVCache`` holds keys and values of all layers in pages, with the tables that say which pages a sequence has.
+A decode step of one layer is ``append`` (norms of queries and keys, position rotation, store of keys and values) and
+``attend`` (attention of the new tokens over the pages), around which a model's projections and its MoE layer
+(``PreparedMoE``) stand; once per step ``extend`` makes room for the new tokens.  ``fork``, ``truncate``, ``free`` and
+``compact`` serve parallel sampling, rolled-back drafts, finished sequences and a pool that is to shrink.
+
+PyTorch supplies device memory and the current stream; all work runs in the sm_100a kernels of the library, on the
+current stream, without host synchronisation (``check_device_status`` excepted).  Argument errors raise before a
+launch; what only the device can see (a page id out of range, a sequence that cannot grow) sets bits of the cache's
+status word, read by ``check_device_status``.  The reference has no attention operator.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import XcbAttnArgs, XcbKvCache, XcbRopeArgs, check
+
+_CACHE_DTYPES = {torch.bfloat16: _lib.XCB_DTYPE_BF16, torch.float16: _lib.XCB_DTYPE_F16,
+                 torch.float8_e4m3fn: _lib.XCB_DTYPE_E4M3}
+_Q_DTYPES = {torch.bfloat16: _lib.XCB_DTYPE_BF16, torch.float16: _lib.XCB_DTYPE_F16}
+
+
+def _check_ints(t: torch.Tensor, n: Optional[int], device: torch.device, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != device:
+        raise ValueError(f"{what} must be int32 [{'n' if n is None else n}] on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+class Rope:
+    """Rotation frequencies of a model: f_i = base^(-2 i / rotary_dim), changed by ``scaling`` for long contexts.
+
+    ``interleaved``: pairs are (2i, 2i + 1), else (i, i + rotary_dim / 2).  ``rotary_dim`` values of each head turn,
+    the rest pass.  ``scaling``: None, or a dict with ``type``
+
+    * ``"linear"``: positions are divided by ``factor``;
+    * ``"ntk"``: the base grows by ``factor^(rotary_dim / (rotary_dim - 2))``;
+    * ``"yarn"``: frequencies that turn more than ``beta_fast`` (32) times within the ``original`` context stay, those
+      that turn less than ``beta_slow`` (1) times are divided by ``factor``, a ramp between; cos and sin are
+      multiplied by ``mscale`` (0.1 ln(factor) + 1).
+
+    Frequencies are kept as 64-bit fractions of a turn, so angles are exact at any position."""
+
+    def __init__(self, rotary_dim: int, *, base: float = 10000.0, interleaved: bool = False,
+                 scaling: Optional[dict] = None, device="cuda"):
+        if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > 256:
+            raise ValueError("rotary_dim must be even, 0 to 256")
+        if not base > 0:
+            raise ValueError("base must be positive")
+        self.rotary_dim, self.base, self.interleaved = int(rotary_dim), float(base), bool(interleaved)
+        self.frequencies, self.mscale = self._frequencies(dict(scaling) if scaling else {})
+        if any(not 0 <= f < 2 * math.pi for f in self.frequencies):
+            raise ValueError("a rotation frequency is not below a full turn per position")
+        words = [min((1 << 64) - 1, int(f / (2 * math.pi) * 2.0 ** 64)) for f in self.frequencies]
+        self.turns = torch.tensor([w - (1 << 64) if w >= 1 << 63 else w for w in words], dtype=torch.int64,
+                                  device=device)
+
+    def _frequencies(self, scaling: dict):
+        rot, base = self.rotary_dim, self.base
+        kind = scaling.pop("type", None)
+        factor = float(scaling.pop("factor", 1.0))
+        if not factor > 0:
+            raise ValueError("the scaling factor must be positive")
+        mscale = 1.0
+        if kind == "ntk":
+            base *= factor ** (rot / max(rot - 2, 1))
+        freqs = [base ** (-2.0 * i / rot) for i in range(rot // 2)]
+        if kind == "linear":
+            freqs = [f / factor for f in freqs]
+        elif kind == "yarn":
+            original = scaling.pop("original")
+            fast, slow = scaling.pop("beta_fast", 32.0), scaling.pop("beta_slow", 1.0)
+            mscale = scaling.pop("mscale", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+
+            def index_of(turns):  # the pair that turns so many times within the original context
+                return rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            low = max(math.floor(index_of(fast)), 0)
+            high = min(math.ceil(index_of(slow)), rot - 1)
+            for i, f in enumerate(freqs):
+                ramp = min(1.0, max(0.0, (i - low) / max(high - low, 0.001)))
+                freqs[i] = f * (1 - ramp) + f / factor * ramp
+        elif kind not in (None, "ntk"):
+            raise ValueError(f"unknown scaling type {kind!r}")
+        if scaling:
+            raise ValueError(f"unknown scaling entries {sorted(scaling)}")
+        return freqs, float(mscale)
+
+
+def _rows(t: torch.Tensor, heads: Optional[int], dim: Optional[int], tokens: Optional[int], what: str) -> torch.Tensor:
+    """[tokens, heads, dim] with contiguous, 16-byte aligned heads; copied where they are not."""
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim) or \
+            (tokens is not None and t.shape[0] != tokens):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    a, b, c = t.stride()
+    if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _norm_weight(w: Optional[torch.Tensor], x: torch.Tensor, what: str):
+    if w is None:
+        return None
+    if w.shape != (x.shape[2],) or w.device != x.device or w.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{what} must be [head_dim], of the queries' type or float32")
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+
+
+def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
+    dtype = _Q_DTYPES.get(q.dtype)
+    if dtype is None or not q.is_cuda:
+        raise ValueError("queries must be bf16 or fp16 CUDA tensors (there is no CPU path)")
+    device = q.device
+    q = _rows(q, None, None, None, "q")
+    tokens, q_heads, dim = q.shape
+    kv_heads = cache.kv_heads if cache is not None else k.shape[1] if k is not None and k.dim() == 3 else 0
+    for t, what in ((k, "k"), (v, "v")):
+        if t is not None and (t.dtype != q.dtype or t.device != device):
+            raise ValueError(f"{what} must have the queries' type and device")
+    k = None if k is None else _rows(k, kv_heads, dim, tokens, "k")
+    v = None if v is None else _rows(v, kv_heads, dim, tokens, "v")
+    if rope.turns.device != device:
+        raise ValueError("rope is on another device than the queries")
+    if rope.rotary_dim > dim:
+        raise ValueError(f"rotary_dim {rope.rotary_dim} is larger than head_dim {dim}")
+    positions = _check_ints(positions, tokens, device, "positions")
+    wq, wk = _norm_weight(q_weight, q, "q_weight"), _norm_weight(k_weight, q, "k_weight")
+    if wq is not None and wk is not None and wq.dtype != wk.dtype:
+        raise ValueError("q_weight and k_weight must have one type")
+    weight = wq if wq is not None else wk
+    outs = []
+    for given, like, what in ((q_out, q, "q_out"), (k_out, k, "k_out")):
+        if given is None:
+            made = torch.empty(like.shape, dtype=q.dtype, device=device) if what == "q_out" or \
+                (cache is None and k is not None) else None
+        else:
+            if like is None or given.shape != like.shape or given.dtype != q.dtype or given.device != device or \
+                    _rows(given, None, None, None, what) is not given:
+                raise ValueError(f"{what} must be like its input, with aligned contiguous heads")
+            made = given
+        outs.append(made)
+    q_out, k_out = outs
+    a = XcbRopeArgs()
+    a.tokens, a.q_heads, a.kv_heads, a.head_dim = tokens, q_heads, kv_heads, dim
+    a.rotary_dim, a.interleaved, a.dtype = rope.rotary_dim, rope.interleaved, dtype
+    a.weight_dtype = dtype if weight is None or weight.dtype == q.dtype else _lib.XCB_DTYPE_F32
+    a.eps, a.weight_offset, a.mscale, a.layer = eps, weight_offset, rope.mscale, layer
+    a.q = q.data_ptr()
+    a.q_stride[:] = q.stride()[:2]
+    a.q_out = q_out.data_ptr()
+    a.q_out_stride[:] = q_out.stride()[:2]
+    if k is not None:
+        a.k = k.data_ptr()
+        a.k_stride[:] = k.stride()[:2]
+    if k_out is not None:
+        a.k_out = k_out.data_ptr()
+        a.k_out_stride[:] = k_out.stride()[:2]
+    if v is not None:
+        a.v = v.data_ptr()
+        a.v_stride[:] = v.stride()[:2]
+    if wq is not None:
+        a.q_weight = wq.data_ptr()
+    if wk is not None:
+        a.k_weight = wk.data_ptr()
+    a.positions, a.turns = positions.data_ptr(), rope.turns.data_ptr()
+    handle = None
+    if cache is not None:
+        seqs = _check_ints(seqs, tokens, device, "seqs")
+        a.seqs, handle = seqs.data_ptr(), cache._address
+    _launch(device, _lib.load().xcb_qk_norm_rope, "xcb_qk_norm_rope", handle, ctypes.addressof(a))
+    return q_out, k_out
+
+
+def _launch(device, fn, what, *args):
+    """Call a C entry on the device's current stream, with that device current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        check(rc, what)
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: Rope, *,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 weight_offset: float = 0.0, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None):
+    """Norms of queries and keys per head and the position rotation, in one pass: ``(q', k')``.
+
+    ``q`` [T, q_heads, D] and ``k`` [T, kv_heads, D] (or None), bf16 or fp16, may be strided views of one projection's
+    rows; ``positions`` int32 [T].  ``q_weight`` / ``k_weight`` [D]: y = x * rsqrt(mean(x^2) + eps) * (w +
+    weight_offset), no norm where None.  ``q_out`` / ``k_out`` may be the inputs themselves."""
+    return _rope_call(None, 0, q, k, None, positions, None, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out)
+
+
+class PagedKVCache:
+    """Keys and values of all layers in pages, and which pages each sequence holds.
+
+    ``kv`` [layers, 2, num_pages, kv_heads, page_size, head_dim] in bf16, fp16 or e4m3; ``page_table`` int32 [max_seqs,
+    max_pages] (-1: no page), ``seq_lens`` int32 [max_seqs], ``refcounts`` int32 [num_pages].  An e4m3 cache holds value
+    / scale, ``k_scale`` and ``v_scale`` fp32 [kv_heads] (None: 1).  The tensors are the state: a caller may copy them,
+    set them back, or share them with its own code.  Calls on one cache must be ordered."""
+
+    def __init__(self, layers: int, num_pages: int, kv_heads: int, page_size: int, head_dim: int, *, max_seqs: int,
+                 max_pages: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        if dtype not in _CACHE_DTYPES:
+            raise ValueError("the cache holds bf16, fp16 or e4m3")
+        if min(layers, num_pages, kv_heads, page_size, head_dim, max_seqs, max_pages) <= 0:
+            raise ValueError("cache sizes must be positive")
+        self._bind(torch.empty((layers, 2, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device),
+                   torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(max_seqs, dtype=torch.int32, device=device),
+                   torch.zeros(num_pages, dtype=torch.int32, device=device), k_scale, v_scale)
+
+    @classmethod
+    def from_tensors(cls, kv: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                     refcounts: Optional[torch.Tensor] = None, *, k_scale: Optional[torch.Tensor] = None,
+                     v_scale: Optional[torch.Tensor] = None) -> "PagedKVCache":
+        """A cache over tensors that the caller holds.  Without ``refcounts`` they are counted from the table."""
+        self = cls.__new__(cls)
+        if kv.dim() != 6 or kv.shape[1] != 2:
+            raise ValueError("kv must be [layers, 2, num_pages, kv_heads, page_size, head_dim]")
+        if refcounts is None:
+            held = page_table.flatten()
+            held = held.masked_fill((held < 0) | (held >= kv.shape[2]), kv.shape[2]).long()
+            refcounts = torch.zeros(kv.shape[2] + 1, dtype=torch.int32, device=kv.device)
+            refcounts = refcounts.index_add_(0, held, torch.ones_like(held, dtype=torch.int32))[:-1]
+        self._bind(kv, page_table, seq_lens, refcounts, k_scale, v_scale)
+        return self
+
+    def _bind(self, kv, table, lens, refs, k_scale, v_scale):
+        if not kv.is_cuda:
+            raise ValueError("the cache must be on a CUDA device (there is no CPU path)")
+        if kv.dtype not in _CACHE_DTYPES:
+            raise ValueError("the cache holds bf16, fp16 or e4m3")
+        self.device = kv.device
+        self.layers, _, self.num_pages, self.kv_heads, self.page_size, self.head_dim = kv.shape
+        for t, shape, what in ((table, (lens.numel(), table.shape[-1]), "page_table"), (lens, (table.shape[0],), "seq_lens"),
+                               (refs, (self.num_pages,), "refcounts")):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"{what} must be contiguous int32 {shape} on {self.device}")
+        if not kv.is_contiguous():
+            raise ValueError("kv must be contiguous")
+        scales = []
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is not None:
+                if kv.dtype != torch.float8_e4m3fn:
+                    raise ValueError(f"{what} belongs to an e4m3 cache")
+                if t.dtype != torch.float32 or tuple(t.shape) != (self.kv_heads,) or t.device != self.device:
+                    raise ValueError(f"{what} must be float32 [{self.kv_heads}] on {self.device}")
+                t = t.contiguous()
+            scales.append(t)
+        self.kv, self.page_table, self.seq_lens, self.refcounts = kv, table, lens, refs
+        self.k_scale, self.v_scale = scales
+        self.max_seqs, self.max_pages = table.shape
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.lib = _lib.load()
+        self._struct = XcbKvCache(self.layers, self.num_pages, self.kv_heads, self.page_size, self.head_dim,
+                                  _CACHE_DTYPES[kv.dtype], self.max_seqs, self.max_pages, kv.data_ptr(),
+                                  table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+                                  None if scales[0] is None else scales[0].data_ptr(),
+                                  None if scales[1] is None else scales[1].data_ptr(), self.status.data_ptr())
+        self._address = ctypes.addressof(self._struct)
+        self._attn_ws: dict = {}
+        self._page_ws: dict = {}
+        if self.lib.xcb_kv_workspace_bytes(self._address) == 0:
+            raise ValueError("unsupported cache shape (head_dim * element bytes must be a multiple of 16, at most 256 "
+                             "values)")
+
+    # -------------------------------------------------------------------------------------- workspaces
+    def _attn_workspace(self, q_heads: int, new_tokens: int) -> torch.Tensor:
+        """The current stream's workspace for this group and token count (counters and partial results)."""
+        key = (torch.cuda.current_stream(self.device).cuda_stream, q_heads, new_tokens)
+        ws = self._attn_ws.get(key)
+        if ws is None:
+            with torch.cuda.device(self.device):
+                nbytes = self.lib.xcb_attn_workspace_bytes(self._address, q_heads, new_tokens)
+            if nbytes == 0:
+                raise ValueError(f"unsupported heads: {q_heads} query heads over {self.kv_heads}, {new_tokens} new tokens")
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            _launch(self.device, self.lib.xcb_attn_workspace_init, "xcb_attn_workspace_init", ws.data_ptr(), nbytes)
+            self._attn_ws[key] = ws
+        return ws
+
+    def _page_workspace(self) -> torch.Tensor:
+        key = torch.cuda.current_stream(self.device).cuda_stream
+        ws = self._page_ws.get(key)
+        if ws is None:
+            nbytes = self.lib.xcb_kv_workspace_bytes(self._address)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            _launch(self.device, self.lib.xcb_kv_workspace_init, "xcb_kv_workspace_init", self._address, ws.data_ptr(),
+                    nbytes)
+            self._page_ws[key] = ws
+        return ws
+
+    # -------------------------------------------------------------------------------------- one layer's step
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+               seqs: torch.Tensor, rope: Rope, *, q_weight: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, weight_offset: float = 0.0,
+               q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Norm and turn ``q`` and ``k`` as ``qk_norm_rope`` does, store k and ``v`` at ``positions`` of sequences
+        ``seqs`` (int32 [T]; -1: padding, not stored) in ``layer``'s pages, and return the turned queries.  The pages
+        must have been given to the sequences by ``extend``."""
+        if k is None or v is None:
+            raise ValueError("append needs keys and values")
+        if q.dim() == 3 and q.shape[2] != self.head_dim:
+            raise ValueError(f"head_dim is {self.head_dim}")
+        if q.device != self.device:
+            raise ValueError("the queries are on another device than the cache")
+        if self.kv.dtype != torch.float8_e4m3fn and q.dtype != self.kv.dtype:
+            raise ValueError("the cache holds another type than the keys")
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        return _rope_call(self, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
+                          None)[0]
+
+    def attend(self, layer: int, q: torch.Tensor, *, seqs: Optional[torch.Tensor] = None, window: int = 0,
+               scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+        """Attention of new tokens over ``layer``'s pages.
+
+        ``q`` [B, L, q_heads, D] (or [B, q_heads, D]: one token each): the last L tokens of sequences ``seqs`` (int32
+        [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
+        ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
+        natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
+        dtype = _Q_DTYPES.get(q.dtype)
+        if dtype is None or q.device != self.device:
+            raise ValueError(f"queries must be bf16 or fp16 on {self.device}")
+        single = q.dim() == 3
+        if single:
+            q = q.unsqueeze(1)
+        if q.dim() != 4 or q.shape[3] != self.head_dim:
+            raise ValueError(f"queries must be [batch, new_tokens, heads, {self.head_dim}]")
+        if self.kv.dtype != torch.float8_e4m3fn and q.dtype != self.kv.dtype:
+            raise ValueError("the cache holds another type than the queries")
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        if window < 0:
+            raise ValueError("window must be >= 0")
+        batch, new, heads, dim = q.shape
+        if heads == 0 or heads % self.kv_heads or new == 0:
+            raise ValueError(f"query heads must be a multiple of {self.kv_heads}, new tokens at least 1")
+        s = q.stride()
+        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            s = q.stride()
+        if seqs is not None:
+            seqs = _check_ints(seqs, batch, self.device, "seqs")
+        elif batch > self.max_seqs:
+            raise ValueError(f"the cache has {self.max_seqs} sequences")
+        shape = (batch, heads, dim) if single else (batch, new, heads, dim)
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError(f"out must be contiguous {shape}, of the queries' type")
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
+        if batch:
+            a = XcbAttnArgs(batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else scale,
+                            q.data_ptr(), s[:3], out.data_ptr(), None if lse is None else lse.data_ptr(),
+                            None if seqs is None else seqs.data_ptr())
+            ws = self._attn_workspace(heads, new)
+            _launch(self.device, self.lib.xcb_paged_attention, "xcb_paged_attention", self._address,
+                    ctypes.addressof(a), ws.data_ptr(), ws.numel())
+        return (out, lse) if return_lse else out
+
+    # -------------------------------------------------------------------------------------- pages
+    def _list(self, t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
+        t = _check_ints(t, n, self.device, what)
+        if n is None and t.shape[0] > self.max_seqs:
+            raise ValueError(f"{what} lists more sequences than the cache has")
+        return t
+
+    def extend(self, seqs: torch.Tensor, new_tokens: torch.Tensor) -> None:
+        """Room for ``new_tokens[i]`` more tokens in sequence ``seqs[i]`` (int32 [n] each); ``seq_lens`` grows.
+
+        The lowest free pages go to the sequences in list order.  A part-full last page that is shared with another
+        sequence is replaced by a copy, so that ``append`` never writes to a shared page; where all its holders grow
+        in one call the first keeps it.  Too few free pages: nothing changes and XCB_STATUS_NO_PAGES is set."""
+        seqs = self._list(seqs, None, "seqs")
+        new_tokens = self._list(new_tokens, seqs.shape[0], "new_tokens")
+        ws = self._page_workspace()
+        _launch(self.device, self.lib.xcb_kv_extend, "xcb_kv_extend", self._address, seqs.data_ptr(),
+                new_tokens.data_ptr(), seqs.shape[0], ws.data_ptr(), ws.numel())
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Sequence ``dst[i]``, empty before, becomes a copy of ``src[i]`` that shares its pages."""
+        src = self._list(src, None, "src")
+        dst = self._list(dst, src.shape[0], "dst")
+        _launch(self.device, self.lib.xcb_kv_fork, "xcb_kv_fork", self._address, src.data_ptr(), dst.data_ptr(),
+                src.shape[0])
+
+    def truncate(self, seqs: torch.Tensor, lens: torch.Tensor) -> None:
+        """Sequence ``seqs[i]`` keeps its first ``lens[i]`` tokens; pages that no sequence holds any more are free."""
+        seqs = self._list(seqs, None, "seqs")
+        lens = self._list(lens, seqs.shape[0], "lens")
+        _launch(self.device, self.lib.xcb_kv_truncate, "xcb_kv_truncate", self._address, seqs.data_ptr(),
+                lens.data_ptr(), seqs.shape[0])
+
+    def free(self, seqs: torch.Tensor) -> None:
+        """The sequences become empty."""
+        seqs = self._list(seqs, None, "seqs")
+        _launch(self.device, self.lib.xcb_kv_truncate, "xcb_kv_truncate", self._address, seqs.data_ptr(), None,
+                seqs.shape[0])
+
+    def compact(self) -> None:
+        """Live pages move down into the free ids below them; the upper part of the pool is free afterwards."""
+        ws = self._page_workspace()
+        _launch(self.device, self.lib.xcb_kv_compact, "xcb_kv_compact", self._address, ws.data_ptr(), ws.numel())
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Contents of page ``src[i]`` to page ``dst[i]`` in all layers (no dst twice, none that is also a src)."""
+        src = _check_ints(src, None, self.device, "src")
+        dst = _check_ints(dst, src.shape[0], self.device, "dst")
+        if src.shape[0] > self.num_pages:
+            raise ValueError("more pairs than pages")
+        _launch(self.device, self.lib.xcb_kv_copy_pages, "xcb_kv_copy_pages", self._address, src.data_ptr(),
+                dst.data_ptr(), src.shape[0])
+
+    def check_device_status(self) -> int:
+        """Synchronise the current stream and return (and clear) the cache's device status bits."""
+        v = ctypes.c_int32(0)
+        with torch.cuda.device(self.device):
+            rc = self.lib.xcb_kv_read_status(self._address, ctypes.addressof(v),
+                                             torch.cuda.current_stream(self.device).cuda_stream)
+        if rc not in (_lib.XCB_OK, _lib.XCB_ERR_DEVICE):
+            check(rc, "xcb_kv_read_status")
+        return v.value
