@@ -35,7 +35,11 @@ def _cache(**kw):
 
 def test_cache_shapes():
     lib = _lib.load()
-    size = lambda **kw: lib.xcb_kv_workspace_bytes(ctypes.addressof(_cache(**kw)))  # noqa: E731
+
+    def size(**kw):
+        c = _cache(**kw)
+        return lib.xcb_kv_workspace_bytes(ctypes.addressof(c))
+
     assert size() > 0
     assert size(num_pages=16) > size()
     for bad in (dict(layers=0), dict(num_pages=-1), dict(kv_heads=0), dict(page_size=0), dict(head_dim=0),

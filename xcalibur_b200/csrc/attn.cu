@@ -43,6 +43,10 @@ struct AttnParams {
   float* part_o;                // [2 * blocks][16 * WM][DP]
 };
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the rest of the 16 bytes is zeroed; with bytes = 0 nothing is read
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -75,11 +79,11 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two e4m3 codes (the low 16 bits) to two f16, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v) {
-  uint32_t r;
-  asm("{\n .reg .b16 h;\n cvt.u16.u32 h, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(v));
-  return r;
+// Four e4m3 codes to two pairs of f16, exactly.
+__device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -94,7 +98,8 @@ struct Shape {
   static constexpr int kWarps = DP == 256 ? 4 : 8;
   static constexpr int kPitch = DP * (F8 ? 1 : 2);   // bytes of one position's row in shared memory
   static constexpr int kChunks = kPitch / 16;
-  static constexpr int kSub = 16 * kPitch;           // keys (or values) of 16 positions
+  static constexpr int kTok = kPitch <= 128 ? 32 : 16;  // positions of a warp's step: 4 to 8 KB of keys and values
+  static constexpr int kSub = kTok * kPitch;         // their keys (or values)
   static constexpr int kFit = 196608 / (kWarps * 2 * kSub);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kRing = kWarps * kStages * 2 * kSub;
@@ -102,7 +107,8 @@ struct Shape {
   static constexpr int kRed = kWarps / 2 * 16 * kRedPitch * 4;
   static constexpr int kRedMl = kWarps / 2 * 16 * 2 * 4;
   static constexpr int kMasks = kWarps * kStages * 4;
-  static constexpr int kBytes = kRing + kRed + kRedMl + kMasks;
+  static constexpr int kScalars = kWarps * 8 + 16;
+  static constexpr int kBytes = kRing + kRed + kRedMl + kMasks + kScalars;
 };
 
 // Byte offset of 16-byte chunk c of row r: rows that ldmatrix reads together fall into different banks.
@@ -115,11 +121,10 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
 struct Seg {
   int b, j, row;        // sequence of the batch; head * row_tiles + tile; row of the page table
   int len, c0, c1, nch; // visible end; chunks [c0, c1) of nch
-  int t0, t1;           // positions of these chunks
+  int t0, t1, lo;       // positions of these chunks; the first that any row sees
   int left;             // chunks of the block's run after this segment
 };
 
-template <int CH>
 __device__ __forceinline__ int visible(const AttnParams& p, int b, int* row, int* lo) {
   const int s = p.seqs ? p.seqs[b] : b;
   int len = 0;
@@ -132,29 +137,29 @@ __device__ __forceinline__ int visible(const AttnParams& p, int b, int* row, int
   *lo = p.window ? (int)max((int64_t)0, (int64_t)len - p.new_tokens + 1 - p.window) : 0;
   return len;
 }
-template <int CH>
+// Chunks are counted from the step that holds the first visible position.
+template <int CH, int TOK>
 __device__ __forceinline__ int chunks_of(int len, int lo) {
-  return max(1, (len - lo + CH - 1) / CH);  // an empty sequence is one empty chunk: its rows are written too
+  return max(1, (len - lo / TOK * TOK + CH - 1) / CH);  // an empty sequence is one empty chunk: its rows are written too
 }
-template <int CH>
+template <int CH, int TOK>
 __device__ __forceinline__ void open_seg(const AttnParams& p, Seg& s, int c0, int units) {
-  int lo;
-  s.len = visible<CH>(p, s.b, &s.row, &lo);
-  s.nch = chunks_of<CH>(s.len, lo);
+  s.len = visible(p, s.b, &s.row, &s.lo);
+  s.nch = chunks_of<CH, TOK>(s.len, s.lo);
   s.c0 = c0;
   s.c1 = min(s.nch, c0 + units);
   s.left = units - (s.c1 - s.c0);
-  s.t0 = lo + c0 * CH;
-  s.t1 = min(s.len, lo + s.c1 * CH);
+  s.t0 = s.lo / TOK * TOK + c0 * CH;
+  s.t1 = min(s.len, s.lo / TOK * TOK + s.c1 * CH);
 }
-template <int CH>
+template <int CH, int TOK>
 __device__ __forceinline__ bool next_seg(const AttnParams& p, Seg& s) {
   if (s.left <= 0) return false;
   if (++s.j == p.kv.kv_heads * p.row_tiles) {
     s.j = 0;
     if (++s.b >= p.batch) return false;
   }
-  open_seg<CH>(p, s, 0, s.left);
+  open_seg<CH, TOK>(p, s, 0, s.left);
   return true;
 }
 
@@ -162,21 +167,23 @@ template <typename T, bool F8, int DP, int WM>
 __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(const AttnParams p) {
   using S = Shape<DP, F8>;
   constexpr int NW = S::kWarps, WN = NW / WM, NS = S::kStages;
-  constexpr int TT = 16 * WM;       // positions of a group's tile
-  constexpr int CH = 16 * NW;       // positions of a chunk
+  constexpr int TOK = S::kTok, SN = TOK / 8;
+  constexpr int TT = TOK * WM;      // positions of a group's tile
+  constexpr int CH = TOK * NW;      // positions of a chunk
+  constexpr int RT = 16 * WM;       // rows of a row tile
   constexpr int KS = DP / 16;       // 16-wide steps of the head dimension
   constexpr int NT = DP / 8;        // 8-wide column tiles of the output
   using M = typename std::conditional<F8, __half, T>::type;  // operand type of the tensor steps
   static_assert(WM <= NW, "a group has at most the block's warps");
 
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];  // all of the block's shared memory: steps start at multiples of 1 KB
   uint8_t* const ring = smem;
   float* const red = reinterpret_cast<float*>(smem + S::kRing);
   float* const red_ml = reinterpret_cast<float*>(smem + S::kRing + S::kRed);
   uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kRed + S::kRedMl);
-  __shared__ int64_t s_warp[NW];
-  __shared__ int s_start[3];
-  __shared__ int s_last;
+  int64_t* const s_warp = reinterpret_cast<int64_t*>(smem + S::kRing + S::kRed + S::kRedMl + S::kMasks);
+  int* const s_start = reinterpret_cast<int*>(s_warp + NW);  // [3]
+  int& s_last = s_start[3];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = warp / WM, wm = warp % WM;
@@ -192,8 +199,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) {
       int row, lo;
-      const int len = visible<CH>(p, b, &row, &lo);
-      mine += (int64_t)chunks_of<CH>(len, lo) * heads;
+      const int len = visible(p, b, &row, &lo);
+      mine += (int64_t)chunks_of<CH, TOK>(len, lo) * heads;
       if (cta == 0 && (row < 0 || row >= p.kv.max_seqs)) atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
     }
     int64_t incl = mine;
@@ -219,8 +226,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
     if (u0 >= at && u0 < at + mine) {
       for (int b = b0; b < b1; ++b) {
         int row, lo;
-        const int len = visible<CH>(p, b, &row, &lo);
-        const int nch = chunks_of<CH>(len, lo);
+        const int len = visible(p, b, &row, &lo);
+        const int nch = chunks_of<CH, TOK>(len, lo);
         if (u0 < at + (int64_t)nch * heads) {
           s_start[0] = b;
           s_start[1] = (int)((u0 - at) / nch);
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
   Seg ps;
   ps.b = s_start[0];
   ps.j = s_start[1];
-  open_seg<CH>(p, ps, s_start[2], (int)(u1 - u0));
+  open_seg<CH, TOK>(p, ps, s_start[2], (int)(u1 - u0));
   Seg cs = ps;
   int ptile = grp;
   bool more = true;
@@ -246,66 +253,108 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
   uint8_t* const my_ring = ring + warp * (NS * 2 * S::kSub);
   uint32_t* const my_masks = masks + warp * NS;
 
-  int64_t f_off = 0;  // of the tile looked up last: byte offset of position `lane`'s row (lanes 0..15)
-  bool f_ok = false;
+  // Of the step looked up last: which of its positions are there, and the byte offset of the first one's row (where
+  // every step lies inside one page) or of lane's one.
+  const bool in_page = p.kv.page_size % TOK == 0;
+  int64_t f_off = 0;
+  uint32_t f_mask = 0;
   const auto look_up = [&]() {
-    f_ok = false;
+    f_mask = 0;
     while (more && ptile * TT >= ps.t1 - ps.t0) {
-      more = next_seg<CH>(p, ps);
+      more = next_seg<CH, TOK>(p, ps);
       ptile = grp;
     }
     if (!more) return;
-    const int pos = ps.t0 + ptile * TT + wm * 16 + lane;
-    if (lane < 16 && pos < ps.t1) {
-      const int pi = fdiv(pos, p.kv.page_div);
-      const int page = p.kv.table[(int64_t)ps.row * p.kv.max_pages + pi];
-      f_ok = page >= 0 && page < p.kv.num_pages;
-      if (!f_ok) atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
-      const int h = fdiv(ps.j, p.head_div);
-      f_off = (((int64_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size)) * row_bytes;
-    }
+    const int pos0 = ps.t0 + ptile * TT + wm * TOK;
     ptile += WN;
+    const int32_t* const row = p.kv.table + (int64_t)ps.row * p.kv.max_pages;
+    const int pos = in_page ? pos0 : pos0 + lane;
+    const bool in = in_page ? pos0 < ps.t1 : lane < TOK && pos >= ps.lo && pos < ps.t1;
+    bool ok = false;
+    if (in) {
+      const int pi = fdiv(pos, p.kv.page_div);
+      const int page = row[pi];
+      ok = (uint32_t)page < (uint32_t)p.kv.num_pages;
+      if (!ok) atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
+      f_off = (((int64_t)page * p.kv.kv_heads + fdiv(ps.j, p.head_div)) * p.kv.page_size + (pos - pi * p.kv.page_size)) *
+              row_bytes;
+    }
+    if (in_page) {
+      const int from = max(0, ps.lo - pos0), to = min(TOK, ps.t1 - pos0);
+      if (ok) f_mask = (uint32_t)(((1ull << to) - 1) & ~((1ull << from) - 1));
+    } else {
+      f_mask = __ballot_sync(0xffffffffu, ok);
+    }
   };
-  const auto issue = [&](int stage, int64_t off, bool ok) {
-    const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+  // This lane copies chunk lc of rows lr, lr + RPI, ...
+  constexpr int RPI = 32 / S::kChunks, IT = TOK / RPI;
+  const int lc = lane % S::kChunks, lr = lane / S::kChunks;
+  const uint32_t l_dst = smem_u32(my_ring) + swz<S::kPitch>(lr, lc);
+  const int64_t l_src = (int64_t)lr * row_bytes + lc * 16;
+  const auto issue = [&](int stage, int64_t off, uint32_t mask) {
     if (lane == 0) my_masks[stage] = mask;
-    if (mask) {
-      const uint32_t dst = smem_u32(my_ring + stage * (2 * S::kSub));
-      const int c = lane % S::kChunks;
-      const bool in = c * 16 < row_bytes;
+    if (!mask) return;
+    const uint32_t dst = l_dst + stage * (2 * S::kSub);
+    // row lr + i * RPI: the swizzle's exclusive or splits into the lane's part and the step's
+    const auto at = [&](int i) {
+      return (S::kPitch >= 128 ? dst ^ (((i * RPI) & 7) << 4) : dst) + i * RPI * S::kPitch;
+    };
+    const uint8_t* k = p.kv.k + off + l_src;
+    if (in_page && mask == (uint32_t)((1ull << TOK) - 1)) {
+      const uint8_t* v = k + p.kv.plane;
+      if (row_bytes == S::kPitch) {
 #pragma unroll
-      for (int i = 0; i < S::kChunks / 2; ++i) {
-        const int r = lane / S::kChunks + i * (32 / S::kChunks);
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        const bool v = in && ((mask >> r) & 1u);
-        const uint8_t* src = p.kv.k + (v ? o + c * 16 : 0);
-        cp_async16(dst + swz<S::kPitch>(r, c), src, v ? 16 : 0);
-        cp_async16(dst + S::kSub + swz<S::kPitch>(r, c), src + p.kv.plane, v ? 16 : 0);
+        for (int i = 0; i < IT; ++i) cp_async16(at(i), k + i * RPI * S::kPitch);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) cp_async16(at(i) + S::kSub, v + i * RPI * S::kPitch);
+      } else {
+        const int n = lc * 16 < row_bytes ? 16 : 0;
+        const int step = RPI * row_bytes;
+        if (!n) k = v = p.kv.k;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) cp_async16(at(i), n ? k + i * step : k, n);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) cp_async16(at(i) + S::kSub, n ? v + i * step : v, n);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < IT; ++i) {
+        const int r = lr + i * RPI;
+        const int64_t o = in_page ? off + (int64_t)r * row_bytes : __shfl_sync(0xffffffffu, off, r);
+        const bool in = lc * 16 < row_bytes && ((mask >> r) & 1u);
+        const uint8_t* src = p.kv.k + (in ? o + lc * 16 : 0);
+        const uint32_t d = smem_u32(my_ring) + stage * (2 * S::kSub) + swz<S::kPitch>(r, lc);
+        cp_async16(d, src, in ? 16 : 0);
+        cp_async16(d + S::kSub, src + p.kv.plane, in ? 16 : 0);
       }
     }
   };
   {
     int64_t off[NS - 1];
-    bool ok[NS - 1];
+    uint32_t mask[NS - 1];
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
       look_up();
       off[s] = f_off;
-      ok[s] = f_ok;
+      mask[s] = f_mask;
     }
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
-      issue(s, off[s], ok[s]);
+      issue(s, off[s], mask[s]);
       cp_async_commit();
     }
     look_up();
   }
 
+  // ldmatrix row addresses of this lane: keys as (position, dimension) pairs, values transposed
+  const uint32_t k_lane = swz<S::kPitch>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+  const uint32_t v_lane = swz<S::kPitch>(lane & 15, lane >> 4);
+
   // ---- the consuming side ----------------------------------------------------------------------------------------
   int stage = 0, fill = NS - 1;
   int64_t unit = u0;  // first chunk of the current segment
   do {
-    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * TT;
+    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
     // this lane's two rows of the warp's 16
     const T* qrow[2];
     int hi[2], lo[2];
@@ -367,6 +416,19 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         }
       }
     }
+    // Scores are multiplied by to_log2 after the maximum is taken, so it is made positive (and never zero: -inf stays).
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (to_log2[i] < 0.f) {
+        to_log2[i] = -to_log2[i];
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+          qf[kk][i] ^= 0x80008000u;
+          qf[kk][2 + i] ^= 0x80008000u;
+        }
+      }
+      to_log2[i] = fmaxf(to_log2[i], 1e-37f);
+    }
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -377,7 +439,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         __syncwarp();
       else
         named_bar(1 + grp, WM * 32);
-      issue(fill, f_off, f_ok);  // into the stage that the tile before this one was read from
+      issue(fill, f_off, f_mask);  // into the stage that the tile before this one was read from
       cp_async_commit();
       look_up();
 
@@ -387,46 +449,47 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         if (!vm) continue;
         const uint8_t* const base = ring + (grp * WM + sub) * (NS * 2 * S::kSub) + stage * (2 * S::kSub);
         const uint32_t kb = smem_u32(base), vb = kb + S::kSub;
-        const int pos0 = cs.t0 + tile * TT + sub * 16;
-        float s[2][4];
+        const int pos0 = cs.t0 + tile * TT + sub * TOK;
+        float s[SN][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        {
-          const int r = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+        for (int n = 0; n < SN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int b = 0; b < SN / 2; ++b) {
+          // the swizzle again: chunk 2 kk + cc of the lane's row is the lane's address xor 32 kk
+          const uint32_t ka = kb + k_lane + b * 16 * S::kPitch;
           if constexpr (F8) {
 #pragma unroll
             for (int k2 = 0; k2 < KS / 2; ++k2) {
               uint32_t w[4];
-              ldsm4(w, kb + swz<S::kPitch>(r, 2 * k2 + cc));
+              ldsm4(w, ka ^ (k2 << 5));
 #pragma unroll
               for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-                  mma16<M>(s[n], qf[2 * k2 + e], e4m3x2_f16x2(w[2 * n + e]), e4m3x2_f16x2(w[2 * n + e] >> 16));
+                for (int n = 0; n < 2; ++n) {
+                  uint32_t b0, b1;
+                  e4m3_f16(w[2 * n + e], b0, b1);
+                  mma16<M>(s[2 * b + n], qf[2 * k2 + e], b0, b1);
+                }
             }
           } else {
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
               uint32_t w[4];
-              ldsm4(w, kb + swz<S::kPitch>(r, 2 * kk + cc));
-              mma16<M>(s[0], qf[kk], w[0], w[1]);
-              mma16<M>(s[1], qf[kk], w[2], w[3]);
+              ldsm4(w, ka ^ (kk << 5));
+              mma16<M>(s[2 * b], qf[kk], w[0], w[1]);
+              mma16<M>(s[2 * b + 1], qf[kk], w[2], w[3]);
             }
           }
         }
         // visible to some rows only: the last new_tokens - 1 positions and the window's edge
-        const bool ragged = p.new_tokens > 1 && (pos0 + 16 > cs.len - p.new_tokens + 1 ||
+        const bool ragged = p.new_tokens > 1 && (pos0 + TOK > cs.len - p.new_tokens + 1 ||
                                                  (p.window && pos0 < cs.len - p.window));
         const auto seen = [&](int col, int i) {
           return ((vm >> col) & 1u) && (!ragged || (pos0 + col < hi[i] && pos0 + col >= lo[i]));
         };
+        if (ragged || vm != (uint32_t)((1ull << TOK) - 1)) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[n][c] *= to_log2[c >> 1];
-        if (ragged || vm != 0xffffu) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < SN; ++n)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               if (!seen(n * 8 + 2 * t + (c & 1), c >> 1)) s[n][c] = -INFINITY;
@@ -434,9 +497,11 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         float mx[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          mx[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+          mx[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+          for (int n = 1; n < SN; ++n) mx[i] = fmaxf(mx[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * to_log2[i];
         }
         if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
           float a[2];
@@ -457,10 +522,10 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         }
         const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[n][c] = ex2(s[n][c] - mm[c >> 1]);
+            s[n][c] = ex2(fmaf(s[n][c], to_log2[c >> 1], -mm[c >> 1]));
             l[c >> 1] += s[n][c];
           }
         // A value that is not finite at a position hidden from some rows would reach them as 0 * inf: such a tile is
@@ -469,23 +534,34 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         if (ragged) {
           bool bad = false;
 #pragma unroll 1
-          for (int i = lane; i < S::kSub / 4; i += 32) {
-            const uint32_t v = reinterpret_cast<const uint32_t*>(base + S::kSub)[i];
-            if constexpr (F8) {
+          for (int i = lane; i < S::kSub / 16; i += 32) {
+            const uint4 v4 = reinterpret_cast<const uint4*>(base + S::kSub)[i];
+            const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-              for (int q = 0; q < 4; ++q) bad |= ((v >> (8 * q)) & 0x7fu) == 0x7fu;
-            } else {
-              constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-              bad |= (v & E) == E || ((v >> 16) & E) == E;
+            for (int q = 0; q < 4; ++q) {
+              if constexpr (F8) {
+                // a byte with all seven low bits set carries into its eighth
+                bad |= (((v[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+              } else {
+                constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+                bad |= (v[q] & E) == E || ((v[q] >> 16) & E) == E;
+              }
             }
           }
           odd = __any_sync(0xffffffffu, bad);
         }
         if (odd) {
 #pragma unroll 1
-          for (int col = 0; col < 16; ++col) {
-            const float mine0 = (col & 8) ? ((col & 1) ? s[1][1] : s[1][0]) : ((col & 1) ? s[0][1] : s[0][0]);
-            const float mine1 = (col & 8) ? ((col & 1) ? s[1][3] : s[1][2]) : ((col & 1) ? s[0][3] : s[0][2]);
+          for (int col = 0; col < TOK; ++col) {
+            float mine0 = 0.f, mine1 = 0.f;
+#pragma unroll
+            for (int n = 0; n < SN; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if ((col >> 3) == n && (col & 1) == e) {
+                  mine0 = s[n][e];
+                  mine1 = s[n][2 + e];
+                }
             const int from = (lane & ~3) | ((col & 7) >> 1);
             const float p0 = __shfl_sync(0xffffffffu, mine0, from), p1 = __shfl_sync(0xffffffffu, mine1, from);
             const bool see0 = seen(col, 0), see1 = seen(col, 1);
@@ -497,9 +573,11 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
                 const int byte = d * (F8 ? 1 : 2);
                 const uint8_t* at = base + S::kSub + swz<S::kPitch>(col, byte >> 4) + (byte & 15);
                 float v;
-                if constexpr (F8)
-                  v = unpack2<__half>(e4m3x2_f16x2(*at)).x;
-                else
+                if constexpr (F8) {
+                  uint32_t f, unused;
+                  e4m3_f16(*at, f, unused);
+                  v = unpack2<__half>(f).x;
+                } else
                   v = unpack2<T>(*reinterpret_cast<const uint16_t*>(at)).x;
                 if (see0) o[n][e] += p0 * v;
                 if (see1) o[n][2 + e] += p1 * v;
@@ -510,31 +588,36 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         // The probabilities as operands.  Rounded once to 16 bits they would add an error as large as the output's own
         // rounding; for a 16-bit cache a second operand carries the rest.  An 8-bit cache's own rounding is coarser by
         // far, and one f16 operand serves.
-        uint32_t a_hi[4], a_lo[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = s[i >> 1][2 * (i & 1)], y = s[i >> 1][2 * (i & 1) + 1];
-          a_hi[i] = pack2<M>(x, y);
-          if constexpr (!F8) {
-            const float2 f = unpack2<M>(a_hi[i]);
-            a_lo[i] = pack2<M>(x - f.x, y - f.y);
+        for (int b = 0; b < SN / 2; ++b) {
+          uint32_t a_hi[4], a_lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = s[2 * b + (i >> 1)][2 * (i & 1)], y = s[2 * b + (i >> 1)][2 * (i & 1) + 1];
+            a_hi[i] = pack2<M>(x, y);
+            if constexpr (!F8) {
+              const float2 f = unpack2<M>(a_hi[i]);
+              a_lo[i] = pack2<M>(x - f.x, y - f.y);
+            }
           }
-        }
-        const int r = (lane & 7) + (lane & 8), cc = lane >> 4;
+          const uint32_t va = vb + v_lane + b * 16 * S::kPitch;
 #pragma unroll
-        for (int n2 = 0; n2 < S::kChunks / 2; ++n2) {
-          uint32_t w[4];
-          ldsm4_trans(w, vb + swz<S::kPitch>(r, 2 * n2 + cc));
+          for (int n2 = 0; n2 < S::kChunks / 2; ++n2) {
+            uint32_t w[4];
+            ldsm4_trans(w, va ^ (n2 << 5));
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if constexpr (F8) {
-              // bytes: position 2t (d, d+1), position 2t+1 (d, d+1): regroup by d
-              const uint32_t even = __byte_perm(w[2 * e], w[2 * e + 1], 0x6420), od = __byte_perm(w[2 * e], w[2 * e + 1], 0x7531);
-              mma16<M>(o[4 * n2 + 2 * e], a_hi, e4m3x2_f16x2(even), e4m3x2_f16x2(even >> 16));
-              mma16<M>(o[4 * n2 + 2 * e + 1], a_hi, e4m3x2_f16x2(od), e4m3x2_f16x2(od >> 16));
-            } else {
-              mma16<M>(o[2 * n2 + e], a_hi, w[2 * e], w[2 * e + 1]);
-              mma16<M>(o[2 * n2 + e], a_lo, w[2 * e], w[2 * e + 1]);
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (F8) {
+                // bytes: position 2t (d, d+1), position 2t+1 (d, d+1): regroup by d
+                uint32_t b0, b1, c0, c1;
+                e4m3_f16(__byte_perm(w[2 * e], w[2 * e + 1], 0x6420), b0, b1);
+                e4m3_f16(__byte_perm(w[2 * e], w[2 * e + 1], 0x7531), c0, c1);
+                mma16<M>(o[4 * n2 + 2 * e], a_hi, b0, b1);
+                mma16<M>(o[4 * n2 + 2 * e + 1], a_hi, c0, c1);
+              } else {
+                mma16<M>(o[2 * n2 + e], a_hi, w[2 * e], w[2 * e + 1]);
+                mma16<M>(o[2 * n2 + e], a_lo, w[2 * e], w[2 * e + 1]);
+              }
             }
           }
         }
@@ -618,8 +701,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
           }
           if (p.lse && t == 0) p.lse[at] = l[i] == 0.f ? -INFINITY : m[i] * 0.6931471805599453f + logf(l[i]);
         } else {
-          float* po = p.part_o + ((int64_t)slot * TT + rl) * DP;
-          if (t == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * TT + rl) * 2) = make_float2(m[i], l[i]);
+          float* po = p.part_o + ((int64_t)slot * RT + rl) * DP;
+          if (t == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(m[i], l[i]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if constexpr (F8) {
@@ -646,13 +729,15 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         __threadfence();
         if (tid == 0) p.counters[first] = 0;
         const int parts = last - first + 1;
-        const auto slot_of = [&](int c) { return 2 * c + (c * total / blocks < a ? 1 : 0); };
-        const int nrows = min(TT, p.rows - tile0);
+        // every block's part is that of its first chunk, but perhaps the first block's
+        const int first_slot = 2 * first + (first * total / blocks < a ? 1 : 0);
+        const auto slot_of = [&](int c) { return c == first ? first_slot : 2 * c; };
+        const int nrows = min(RT, p.rows - tile0);
         constexpr int W = DP / 32;
         for (int rl = warp; rl < nrows; rl += NW) {
           float top = -INFINITY;
           for (int q = lane; q < parts; q += 32)
-            top = fmaxf(top, __ldcg(p.part_ml + ((int64_t)slot_of(first + q) * TT + rl) * 2));
+            top = fmaxf(top, __ldcg(p.part_ml + ((int64_t)slot_of(first + q) * RT + rl) * 2));
 #pragma unroll
           for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
           float sum = 0.f, acc[W];
@@ -662,7 +747,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
             float wt = 0.f;
             if (q0 + lane < parts) {
               const float2 ml =
-                  __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot_of(first + q0 + lane) * TT + rl) * 2));
+                  __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot_of(first + q0 + lane) * RT + rl) * 2));
               wt = ex2_diff(ml.x, top);
               sum += wt * ml.y;
             }
@@ -670,7 +755,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
 #pragma unroll 8
             for (int q = 0; q < n; ++q) {
               const float wq = __shfl_sync(0xffffffffu, wt, q);
-              const float* src = p.part_o + ((int64_t)slot_of(first + q0 + q) * TT + rl) * DP + lane * W;
+              const float* src = p.part_o + ((int64_t)slot_of(first + q0 + q) * RT + rl) * DP + lane * W;
               if constexpr (W == 2) {
                 const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
                 acc[0] += wq * v.x;
@@ -701,7 +786,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
       }
     }
     unit += cs.c1 - cs.c0;
-  } while (next_seg<CH>(p, cs));
+  } while (next_seg<CH, TOK>(p, cs));
   cp_async_wait<0>();
 }
 
@@ -731,7 +816,7 @@ AttnWs attn_ws(int sms, int wm, int dp) {
 template <typename T, bool F8, int DP, int WM>
 int launch(const AttnParams& p, int sms, cudaStream_t stream) {
   constexpr int bytes = Shape<DP, F8>::kBytes;
-  static_assert(bytes + 1024 <= 227 * 1024, "the stages fit one SM");
+  static_assert(bytes <= 227 * 1024, "the stages fit one SM");
   static bool ready[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return XCB_ERR_CUDA;
