@@ -14,47 +14,31 @@
 // several runs is joined by the block that finishes it last, in run order whoever that is, so results do not depend on
 // timing.
 //
-// Inside a block every group of WM warps streams its own 16 * WM positions through its own ring of shared-memory
-// stages (cp.async, 16 bytes a lane, swizzled so that ldmatrix has no bank conflicts); with WM = 1 (up to 16 rows)
-// warps never wait for one another but at the end of a (sequence, head).  WM = 2, 4, 8 spread up to 128 rows over
-// the warps of a group, which share the stages.
-#include <math.h>
-
+// Inside a block two producer warps copy chunk after chunk into a ring of shared-memory stages (cp.async, 16 bytes a
+// lane, swizzled so that ldmatrix has no bank conflicts, positions that are not there as zeros) and run ahead over the
+// ends of segments; up to eight consumer warps compute.  Consumers are WN groups of WM warps: a group takes its share
+// of a chunk's positions, the warps of a group 16 rows each (WM = 1, 2, 4, 8 for up to 128 rows).  Stages pass between
+// the two by mbarriers alone; groups meet at the end of a segment, where the rows' parts are joined.
+//
+// mma.sync m16n8k16 rather than tcgen05: with 16 rows a 16-bit chunk asks for an eighth of the former's rate, the rows
+// are the M of its step as they are, and its accumulators stay in the registers that the softmax needs them in.
+//
+// Waits are bounded: one that runs out sets XCB_STATUS_DEVICE_TIMEOUT and a flag under which no wait waits and no copy
+// is issued any more, and every warp runs to its end.
 #include <type_traits>
 
-#include "common.cuh"
-#include "kv.cuh"
+#include "attn_split.cuh"
 
 namespace xcb {
 namespace {
 
-struct AttnParams {
-  KvLayer kv;
-  const void* q;
-  int64_t q_b, q_t, q_h;
-  void* out;
-  float* lse;
-  const int32_t* seqs;
-  int32_t batch, new_tokens, group, q_heads, rows, row_tiles, dim, window;
-  float scale_log2;
-  FastDiv group_div, head_div;  // head_div: by row_tiles
-  int32_t* counters;            // [blocks], zero between calls
-  float* part_ml;               // [2 * blocks][16 * WM][2]
-  float* part_o;                // [2 * blocks][16 * WM][DP]
-};
+constexpr uint64_t kWaitNs = 2000000000ull;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 // the rest of the 16 bytes is zeroed; with bytes = 0 nothing is read
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -85,30 +69,27 @@ __device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi)
       : "=r"(lo), "=r"(hi)
       : "r"(v));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// e^(a - b) in base 2 where b is a maximum that may be -inf (nothing seen yet)
-__device__ __forceinline__ float ex2_diff(float a, float b) { return ex2(a - (b == -INFINITY ? 0.f : b)); }
-
 template <int DP, bool F8>
 struct Shape {
-  static constexpr int kWarps = DP == 256 ? 4 : 8;
+  static constexpr int kWarps = DP == 256 ? 4 : 8;   // consumers
+  static constexpr int kProducers = 2;
+  static constexpr int kThreads = (kWarps + kProducers) * 32;
   static constexpr int kPitch = DP * (F8 ? 1 : 2);   // bytes of one position's row in shared memory
   static constexpr int kChunks = kPitch / 16;
   static constexpr int kTok = kPitch <= 128 ? 32 : 16;  // positions of a warp's step: 4 to 8 KB of keys and values
-  static constexpr int kSub = kTok * kPitch;         // their keys (or values)
-  static constexpr int kFit = 196608 / (kWarps * 2 * kSub);
+  static constexpr int kCh = kTok * kWarps;          // positions of a chunk
+  static constexpr int kHalf = kCh * kPitch;         // a stage: its keys, then its values
+  static constexpr int kFit = 196608 / (2 * kHalf);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kRing = kWarps * kStages * 2 * kSub;
-  static constexpr int kRedPitch = DP + 4;
-  static constexpr int kRed = kWarps / 2 * 16 * kRedPitch * 4;
-  static constexpr int kRedMl = kWarps / 2 * 16 * 2 * 4;
-  static constexpr int kMasks = kWarps * kStages * 4;
-  static constexpr int kScalars = kWarps * 8 + 16;
-  static constexpr int kBytes = kRing + kRed + kRedMl + kMasks + kScalars;
+  static constexpr int kRing = kStages * 2 * kHalf;
+  static constexpr int kRedPitch = DP + 8;           // floats
+  static constexpr int kSlots = kWarps / 2;
+  static constexpr int kRed = kSlots * 16 * kRedPitch * 4;
+  static constexpr int kRedMl = kSlots * 16 * 2 * 4;
+  static constexpr int kBars = 2 * kStages * 8;
+  static constexpr int kMasks = kStages * (kCh / 32) * 4;
+  static constexpr int kScalars = 16 * 4;            // sums of the warps, then: place of the run's start, two flags
+  static constexpr int kBytes = kRing + kRed + kRedMl + kBars + kMasks + kScalars;
 };
 
 // Byte offset of 16-byte chunk c of row r: rows that ldmatrix reads together fall into different banks.
@@ -117,278 +98,189 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
   return r * PITCH + ((PITCH >= 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
 }
 
-// A run of chunks of one (sequence, kv head, row tile).
-struct Seg {
-  int b, j, row;        // sequence of the batch; head * row_tiles + tile; row of the page table
-  int len, c0, c1, nch; // visible end; chunks [c0, c1) of nch
-  int t0, t1, lo;       // positions of these chunks; the first that any row sees
-  int left;             // chunks of the block's run after this segment
-};
-
-__device__ __forceinline__ int visible(const AttnParams& p, int b, int* row, int* lo) {
-  const int s = p.seqs ? p.seqs[b] : b;
-  int len = 0;
-  if (s >= 0 && s < p.kv.max_seqs) {
-    len = max(0, p.kv.lens[s]);
-    len = (int)min((int64_t)len, (int64_t)p.kv.max_pages * p.kv.page_size);
-  }
-  *row = s;
-  // the first new token stands at len - new_tokens and sees back to there + 1 - window
-  *lo = p.window ? (int)max((int64_t)0, (int64_t)len - p.new_tokens + 1 - p.window) : 0;
-  return len;
-}
-// Chunks are counted from the step that holds the first visible position.
-template <int CH, int TOK>
-__device__ __forceinline__ int chunks_of(int len, int lo) {
-  return max(1, (len - lo / TOK * TOK + CH - 1) / CH);  // an empty sequence is one empty chunk: its rows are written too
-}
-template <int CH, int TOK>
-__device__ __forceinline__ void open_seg(const AttnParams& p, Seg& s, int c0, int units) {
-  s.len = visible(p, s.b, &s.row, &s.lo);
-  s.nch = chunks_of<CH, TOK>(s.len, s.lo);
-  s.c0 = c0;
-  s.c1 = min(s.nch, c0 + units);
-  s.left = units - (s.c1 - s.c0);
-  s.t0 = s.lo / TOK * TOK + c0 * CH;
-  s.t1 = min(s.len, s.lo / TOK * TOK + s.c1 * CH);
-}
-template <int CH, int TOK>
-__device__ __forceinline__ bool next_seg(const AttnParams& p, Seg& s) {
-  if (s.left <= 0) return false;
-  if (++s.j == p.kv.kv_heads * p.row_tiles) {
-    s.j = 0;
-    if (++s.b >= p.batch) return false;
-  }
-  open_seg<CH, TOK>(p, s, 0, s.left);
-  return true;
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {  // when this thread's copies so far have landed
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 template <typename T, bool F8, int DP, int WM>
-__global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const AttnParams p) {
   using S = Shape<DP, F8>;
   constexpr int NW = S::kWarps, WN = NW / WM, NS = S::kStages;
   constexpr int TOK = S::kTok, SN = TOK / 8;
-  constexpr int TT = TOK * WM;      // positions of a group's tile
-  constexpr int CH = TOK * NW;      // positions of a chunk
+  constexpr int CH = S::kCh;
   constexpr int RT = 16 * WM;       // rows of a row tile
   constexpr int KS = DP / 16;       // 16-wide steps of the head dimension
   constexpr int NT = DP / 8;        // 8-wide column tiles of the output
   using M = typename std::conditional<F8, __half, T>::type;  // operand type of the tensor steps
-  static_assert(WM <= NW, "a group has at most the block's warps");
+  static_assert(WM <= NW && CH % 64 == 0, "a group has at most the block's warps");
 
-  extern __shared__ __align__(1024) uint8_t smem[];  // all of the block's shared memory: steps start at multiples of 1 KB
+  extern __shared__ __align__(1024) uint8_t smem[];  // all of the block's shared memory: stages start at multiples of 1 KB
   uint8_t* const ring = smem;
   float* const red = reinterpret_cast<float*>(smem + S::kRing);
   float* const red_ml = reinterpret_cast<float*>(smem + S::kRing + S::kRed);
-  uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kRed + S::kRedMl);
-  int64_t* const s_warp = reinterpret_cast<int64_t*>(smem + S::kRing + S::kRed + S::kRedMl + S::kMasks);
-  int* const s_start = reinterpret_cast<int*>(s_warp + NW);  // [3]
-  int& s_last = s_start[3];
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kRing + S::kRed + S::kRedMl);
+  uint64_t* const empty = full + NS;
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(empty + NS);  // [NS][CH / 32]: positions that are there
+  int* const s_sum = reinterpret_cast<int*>(masks + NS * (CH / 32));
+  int* const s_start = s_sum + 11;  // [3]
+  int& s_last = s_sum[14];
+  volatile int* const s_dead = s_sum + 15;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(full + i, S::kProducers * 33);  // every producer lane's copies, and the masks of its warp
+      mbar_init(empty + i, NW);
+    }
+    fence_mbar_init();
+    *s_dead = 0;
+  }
+  Run run;
+  if (!plan_run<CH>(p, TOK, s_sum, s_start, run)) return;  // two block barriers: the set-up above is visible
+
+  const auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!*s_dead && !mbar_wait(bar, parity, kWaitNs, p.kv.status)) *s_dead = 1;
+    __syncwarp();
+  };
+  Seg cs;
+  cs.b = s_start[0];
+  cs.j = s_start[1];
+  open_seg<CH>(p, cs, s_start[2], run.u1 - run.u0, TOK);
+  const int row_bytes = p.dim * (F8 ? 1 : 2);
+
+  if (warp >= NW) {
+    // ---- producers: each warp half of every chunk's positions, 32 at a time -------------------------------------------
+    constexpr int UN = CH / 64, RPI = 32 / S::kChunks;
+    const int half = warp - NW;
+    const int lc = lane % S::kChunks, lr = lane / S::kChunks;  // this lane copies 16 bytes at lc of rows lr, lr + RPI, ..
+    const int n_lane = lc * 16 < row_bytes ? 16 : 0;
+    const uint8_t* const src0 = p.kv.k + (n_lane ? lc * 16 : 0);
+    int ci = 0;
+    bool more = true;
+    uint32_t next[UN];  // row of position `lane` of each 32 in the layer's keys, or ~0
+    const auto look_up = [&]() {
+#pragma unroll
+      for (int u = 0; u < UN; ++u) next[u] = 0xffffffffu;
+      if (!more) return;
+      const int pos0 = cs.t0 + ci * CH + half * (CH / 2) + lane;
+      const int32_t* const row = p.kv.table + (int64_t)cs.row * p.kv.max_pages;
+      const int h = fdiv(cs.j, p.head_div);
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int pos = pos0 + u * 32;
+        if (pos >= cs.lo && pos < cs.t1) {
+          const int pi = fdiv(pos, p.kv.page_div);
+          const int page = row[pi];
+          if ((uint32_t)page < (uint32_t)p.kv.num_pages)
+            next[u] = ((uint32_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size);
+          else
+            atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
+        }
+      }
+      if (++ci == cs.c1 - cs.c0) {
+        more = next_seg<CH>(p, cs, TOK);
+        ci = 0;
+      }
+    };
+    look_up();
+    int stage = 0;
+    uint32_t parity = 1;  // the first round finds the stages empty
+    for (int c = run.u0; c < run.u1; ++c) {
+      uint32_t cur[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) cur[u] = next[u];
+      look_up();  // one chunk before it is needed
+      wait(empty + stage, parity);
+      if (!*s_dead) {
+        const uint32_t dst0 = smem_u32(ring) + stage * (2 * S::kHalf);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int r0 = half * (CH / 2) + u * 32;
+          const uint32_t mask = __ballot_sync(0xffffffffu, cur[u] != 0xffffffffu);
+          if (lane == 0) masks[stage * (CH / 32) + r0 / 32] = mask;
+#pragma unroll 8
+          for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = lr + i * RPI;
+            const uint32_t at = __shfl_sync(0xffffffffu, cur[u], r);
+            const bool in = at != 0xffffffffu;
+            const uint8_t* const src = src0 + (in ? (uint64_t)at * (uint32_t)row_bytes : 0ull);
+            const uint32_t dst = dst0 + swz<S::kPitch>(r0 + r, lc);
+            cp_async16(dst, src, in ? n_lane : 0);
+            cp_async16(dst + S::kHalf, src + p.kv.plane, in ? n_lane : 0);
+          }
+        }
+      }
+      cp_async_arrive(full + stage);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + stage);
+      if (++stage == NS) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+    cp_async_wait_all();
+    return;
+  }
+
+  // ---- consumers -----------------------------------------------------------------------------------------------------
   const int grp = warp / WM, wm = warp % WM;
   const int g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x;
-
-  // ---- this block's run of chunks -------------------------------------------------------------------------------
-  int64_t total, u0, u1;
-  {
-    const int heads = p.kv.kv_heads * p.row_tiles;
-    const int per = (p.batch + NW * 32 - 1) / (NW * 32);
-    const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) {
-      int row, lo;
-      const int len = visible(p, b, &row, &lo);
-      mine += (int64_t)chunks_of<CH, TOK>(len, lo) * heads;
-      if (cta == 0 && (row < 0 || row >= p.kv.max_seqs)) atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < warp) before += s_warp[w];
-      all += s_warp[w];
-    }
-    total = all;
-    const int64_t n = min((int64_t)gridDim.x, total);
-    if (cta >= n) return;
-    u0 = cta * total / n;
-    u1 = (cta + 1) * total / n;
-    int64_t at = before + incl - mine;
-    if (u0 >= at && u0 < at + mine) {
-      for (int b = b0; b < b1; ++b) {
-        int row, lo;
-        const int len = visible(p, b, &row, &lo);
-        const int nch = chunks_of<CH, TOK>(len, lo);
-        if (u0 < at + (int64_t)nch * heads) {
-          s_start[0] = b;
-          s_start[1] = (int)((u0 - at) / nch);
-          s_start[2] = (int)((u0 - at) % nch);
-          break;
-        }
-        at += (int64_t)nch * heads;
-      }
-    }
-    __syncthreads();
-  }
-  const int blocks = (int)min((int64_t)gridDim.x, total);
-
-  // ---- the producing side of a warp: 16 positions per tile -------------------------------------------------------
-  Seg ps;
-  ps.b = s_start[0];
-  ps.j = s_start[1];
-  open_seg<CH, TOK>(p, ps, s_start[2], (int)(u1 - u0));
-  Seg cs = ps;
-  int ptile = grp;
-  bool more = true;
-  const int row_bytes = p.dim * (F8 ? 1 : 2);
-  uint8_t* const my_ring = ring + warp * (NS * 2 * S::kSub);
-  uint32_t* const my_masks = masks + warp * NS;
-
-  // Of the step looked up last: which of its positions are there, and the byte offset of the first one's row (where
-  // every step lies inside one page) or of lane's one.
-  const bool in_page = p.kv.page_size % TOK == 0;
-  int64_t f_off = 0;
-  uint32_t f_mask = 0;
-  const auto look_up = [&]() {
-    f_mask = 0;
-    while (more && ptile * TT >= ps.t1 - ps.t0) {
-      more = next_seg<CH, TOK>(p, ps);
-      ptile = grp;
-    }
-    if (!more) return;
-    const int pos0 = ps.t0 + ptile * TT + wm * TOK;
-    ptile += WN;
-    const int32_t* const row = p.kv.table + (int64_t)ps.row * p.kv.max_pages;
-    const int pos = in_page ? pos0 : pos0 + lane;
-    const bool in = in_page ? pos0 < ps.t1 : lane < TOK && pos >= ps.lo && pos < ps.t1;
-    bool ok = false;
-    if (in) {
-      const int pi = fdiv(pos, p.kv.page_div);
-      const int page = row[pi];
-      ok = (uint32_t)page < (uint32_t)p.kv.num_pages;
-      if (!ok) atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
-      f_off = (((int64_t)page * p.kv.kv_heads + fdiv(ps.j, p.head_div)) * p.kv.page_size + (pos - pi * p.kv.page_size)) *
-              row_bytes;
-    }
-    if (in_page) {
-      const int from = max(0, ps.lo - pos0), to = min(TOK, ps.t1 - pos0);
-      if (ok) f_mask = (uint32_t)(((1ull << to) - 1) & ~((1ull << from) - 1));
-    } else {
-      f_mask = __ballot_sync(0xffffffffu, ok);
-    }
-  };
-  // This lane copies chunk lc of rows lr, lr + RPI, ...
-  constexpr int RPI = 32 / S::kChunks, IT = TOK / RPI;
-  const int lc = lane % S::kChunks, lr = lane / S::kChunks;
-  const uint32_t l_dst = smem_u32(my_ring) + swz<S::kPitch>(lr, lc);
-  const int64_t l_src = (int64_t)lr * row_bytes + lc * 16;
-  const auto issue = [&](int stage, int64_t off, uint32_t mask) {
-    if (lane == 0) my_masks[stage] = mask;
-    if (!mask) return;
-    const uint32_t dst = l_dst + stage * (2 * S::kSub);
-    // row lr + i * RPI: the swizzle's exclusive or splits into the lane's part and the step's
-    const auto at = [&](int i) {
-      return (S::kPitch >= 128 ? dst ^ (((i * RPI) & 7) << 4) : dst) + i * RPI * S::kPitch;
-    };
-    const uint8_t* k = p.kv.k + off + l_src;
-    if (in_page && mask == (uint32_t)((1ull << TOK) - 1)) {
-      const uint8_t* v = k + p.kv.plane;
-      if (row_bytes == S::kPitch) {
-#pragma unroll
-        for (int i = 0; i < IT; ++i) cp_async16(at(i), k + i * RPI * S::kPitch);
-#pragma unroll
-        for (int i = 0; i < IT; ++i) cp_async16(at(i) + S::kSub, v + i * RPI * S::kPitch);
-      } else {
-        const int n = lc * 16 < row_bytes ? 16 : 0;
-        const int step = RPI * row_bytes;
-        if (!n) k = v = p.kv.k;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) cp_async16(at(i), n ? k + i * step : k, n);
-#pragma unroll
-        for (int i = 0; i < IT; ++i) cp_async16(at(i) + S::kSub, n ? v + i * step : v, n);
-      }
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < IT; ++i) {
-        const int r = lr + i * RPI;
-        const int64_t o = in_page ? off + (int64_t)r * row_bytes : __shfl_sync(0xffffffffu, off, r);
-        const bool in = lc * 16 < row_bytes && ((mask >> r) & 1u);
-        const uint8_t* src = p.kv.k + (in ? o + lc * 16 : 0);
-        const uint32_t d = smem_u32(my_ring) + stage * (2 * S::kSub) + swz<S::kPitch>(r, lc);
-        cp_async16(d, src, in ? 16 : 0);
-        cp_async16(d + S::kSub, src + p.kv.plane, in ? 16 : 0);
-      }
-    }
-  };
-  {
-    int64_t off[NS - 1];
-    uint32_t mask[NS - 1];
-#pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-      look_up();
-      off[s] = f_off;
-      mask[s] = f_mask;
-    }
-#pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-      issue(s, off[s], mask[s]);
-      cp_async_commit();
-    }
-    look_up();
-  }
-
   // ldmatrix row addresses of this lane: keys as (position, dimension) pairs, values transposed
   const uint32_t k_lane = swz<S::kPitch>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
   const uint32_t v_lane = swz<S::kPitch>(lane & 15, lane >> 4);
+  const auto block_sync = [&]() {
+    __syncwarp();
+    named_bar(1, NW * 32);
+  };
 
-  // ---- the consuming side ----------------------------------------------------------------------------------------
-  int stage = 0, fill = NS - 1;
-  int64_t unit = u0;  // first chunk of the current segment
-  do {
-    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
-    // this lane's two rows of the warp's 16
-    const T* qrow[2];
-    int hi[2], lo[2];
+  // This lane's two rows of the warp's 16, as they lie in memory.
+  uint32_t qf[KS][4];
+  const auto load_q = [&](const Seg& sg) {
+    const int h = fdiv(sg.j, p.head_div), tile0 = (sg.j - h * p.row_tiles) * RT;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = tile0 + wm * 16 + g + 8 * i;
-      qrow[i] = nullptr;
-      hi[i] = cs.len;
-      lo[i] = 0;
-      if (r < p.rows) {
-        const int l = fdiv(r, p.group_div);
-        qrow[i] = (const T*)p.q + cs.b * p.q_b + l * p.q_t + (h * p.group + r - l * p.group) * p.q_h;
-        hi[i] = cs.len - p.new_tokens + l + 1;
-        lo[i] = p.window ? max(0, hi[i] - p.window) : 0;
-      }
-    }
-    uint32_t qf[KS][4];
-    float to_log2[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
+      const bool in = r < p.rows;
+      const int l = in ? fdiv(r, p.group_div) : 0;
+      const T* const q = (const T*)p.q + (in ? sg.b * p.q_b + l * p.q_t + (h * p.group + r - l * p.group) * p.q_h : 0);
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         if constexpr (F8) {
           // a step's contraction index runs over d = 4t, 4t+1 | 4t+2, 4t+3: the four codes a lane gets of a row
           uint2 v = make_uint2(0, 0);
-          if (qrow[i] && kk * 16 < p.dim) v = *reinterpret_cast<const uint2*>(qrow[i] + kk * 16 + 4 * t);
+          if (in && kk * 16 < p.dim) v = *reinterpret_cast<const uint2*>(q + kk * 16 + 4 * t);
           qf[kk][i] = v.x;
           qf[kk][2 + i] = v.y;
         } else {
-          qf[kk][i] = qrow[i] && kk * 16 < p.dim ? *reinterpret_cast<const uint32_t*>(qrow[i] + kk * 16 + 2 * t) : 0u;
-          qf[kk][2 + i] =
-              qrow[i] && kk * 16 + 8 < p.dim ? *reinterpret_cast<const uint32_t*>(qrow[i] + kk * 16 + 8 + 2 * t) : 0u;
+          qf[kk][i] = in && kk * 16 < p.dim ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 2 * t) : 0u;
+          qf[kk][2 + i] = in && kk * 16 + 8 < p.dim ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8 + 2 * t) : 0u;
         }
       }
+    }
+  };
+  load_q(cs);
+
+  int stage = 0;
+  uint32_t parity = 0;
+  int unit = run.u0;  // first chunk of the current segment
+  for (;;) {
+    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
+    // positions that this lane's two rows see
+    int hi[2], lo[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = tile0 + wm * 16 + g + 8 * i;
+      hi[i] = cs.len;
+      lo[i] = 0;
+      if (p.new_tokens > 1 && r < p.rows) {
+        hi[i] = cs.len - p.new_tokens + fdiv(r, p.group_div) + 1;
+        lo[i] = p.window ? max(0, hi[i] - p.window) : 0;
+      }
+    }
+    float to_log2[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
       to_log2[i] = p.scale_log2;
       if constexpr (F8) {
         if (p.kv.k_scale) to_log2[i] *= p.kv.k_scale[h];
@@ -433,23 +325,19 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
-    for (int tile = grp; tile * TT < cs.t1 - cs.t0; tile += WN) {
-      cp_async_wait<NS - 2>();
-      if constexpr (WM == 1)
-        __syncwarp();
-      else
-        named_bar(1 + grp, WM * 32);
-      issue(fill, f_off, f_mask);  // into the stage that the tile before this one was read from
-      cp_async_commit();
-      look_up();
-
+    const int n_chunks = cs.c1 - cs.c0;
+    for (int ci = 0; ci < n_chunks; ++ci) {
+      wait(full + stage, parity);
+      const uint8_t* const base0 = ring + stage * (2 * S::kHalf);
 #pragma unroll 1
       for (int sub = 0; sub < WM; ++sub) {
-        const uint32_t vm = masks[(grp * WM + sub) * NS + stage];
+        const int first = (grp * WM + sub) * TOK;  // of the chunk's positions
+        const uint32_t word = masks[stage * (CH / 32) + first / 32];
+        const uint32_t vm = TOK == 32 ? word : (word >> (first & 31)) & 0xffffu;
         if (!vm) continue;
-        const uint8_t* const base = ring + (grp * WM + sub) * (NS * 2 * S::kSub) + stage * (2 * S::kSub);
-        const uint32_t kb = smem_u32(base), vb = kb + S::kSub;
-        const int pos0 = cs.t0 + tile * TT + sub * TOK;
+        const uint8_t* const base = base0 + first * S::kPitch;  // values: kHalf further
+        const uint32_t kb = smem_u32(base), vb = kb + S::kHalf;
+        const int pos0 = cs.t0 + ci * CH + first;
         float s[SN][4];
 #pragma unroll
         for (int n = 0; n < SN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -534,8 +422,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
         if (ragged) {
           bool bad = false;
 #pragma unroll 1
-          for (int i = lane; i < S::kSub / 16; i += 32) {
-            const uint4 v4 = reinterpret_cast<const uint4*>(base + S::kSub)[i];
+          for (int i = lane; i < TOK * S::kPitch / 16; i += 32) {
+            const uint4 v4 = reinterpret_cast<const uint4*>(base + S::kHalf)[i];
             const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -571,7 +459,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
               for (int e = 0; e < 2; ++e) {
                 const int d = F8 ? (n >> 1) * 16 + 4 * t + 2 * e + (n & 1) : n * 8 + 2 * t + e;
                 const int byte = d * (F8 ? 1 : 2);
-                const uint8_t* at = base + S::kSub + swz<S::kPitch>(col, byte >> 4) + (byte & 15);
+                const uint8_t* at = base + S::kHalf + swz<S::kPitch>(col, byte >> 4) + (byte & 15);
                 float v;
                 if constexpr (F8) {
                   uint32_t f, unused;
@@ -622,95 +510,156 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
           }
         }
       }
-      stage = stage + 1 == NS ? 0 : stage + 1;
-      fill = fill + 1 == NS ? 0 : fill + 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + stage);
+      if (++stage == NS) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
+    Seg nx = cs;
+    const bool more = next_seg<CH>(p, nx, TOK);
+    if (more) load_q(nx);  // under way while the parts are joined
 
-    // ---- join the block's groups, a tree in fixed order ------------------------------------------------------------
+    // ---- join the block's groups and write -----------------------------------------------------------------------------
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
-    // (row of the warp's 16, columns) of accumulator pair (n, i) are one float2 of the natural order, two strided
-    // floats for an 8-bit cache
-    const auto column = [&](int n, int e) { return F8 ? (n >> 1) * 16 + 4 * t + 2 * e + (n & 1) : n * 8 + 2 * t + e; };
+    const bool whole = cs.c0 == 0 && cs.c1 == cs.nch;
+    const float vs = F8 && p.kv.v_scale ? p.kv.v_scale[h] : 1.f;
+    const int slot = 2 * cta + (unit == run.u0 ? 0 : 1);
+    const int nrows = min(RT, p.rows - tile0);
+    const auto place = [&](int r) {  // of row r of the kv head in the output
+      const int tok = fdiv(r, p.group_div);
+      return ((int64_t)cs.b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
+    };
+    // A warp's part in a slot of the join buffer: rows of kRedPitch floats in the natural order of the dimensions, which
+    // an 8-bit cache's accumulators hold four by four.
+    const auto put = [&](int slot_) {
+      float* const dst = red + slot_ * 16 * S::kRedPitch;
+      float* const ml = red_ml + slot_ * 32;
 #pragma unroll
-    for (int half = WN / 2; half > 0; half >>= 1) {
-      __syncthreads();
-      if (grp >= half && grp < 2 * half) {
-        float* dst = red + ((grp - half) * WM + wm) * 16 * S::kRedPitch;
-        float* ml = red_ml + ((grp - half) * WM + wm) * 32;
+      for (int i = 0; i < 2; ++i) {
+        float* const at = dst + (g + 8 * i) * S::kRedPitch;
+        if (t == 0) *reinterpret_cast<float2*>(ml + 2 * (g + 8 * i)) = make_float2(m[i], l[i]);
+        if constexpr (F8) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (t == 0) *reinterpret_cast<float2*>(ml + 2 * (g + 8 * i)) = make_float2(m[i], l[i]);
+          for (int n = 0; n < NT; n += 2)
+            *reinterpret_cast<float4*>(at + n * 8 + 4 * t) =
+                make_float4(o[n][2 * i], o[n + 1][2 * i], o[n][2 * i + 1], o[n + 1][2 * i + 1]);
+        } else {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            dst[(g + 8 * i) * S::kRedPitch + column(n, 0)] = o[n][2 * i];
-            dst[(g + 8 * i) * S::kRedPitch + column(n, 1)] = o[n][2 * i + 1];
-          }
+          for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(at + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
       }
-      __syncthreads();
-      if (grp < half) {
-        const float* src = red + (grp * WM + wm) * 16 * S::kRedPitch;
-        const float* ml = red_ml + (grp * WM + wm) * 32;
+    };
+    if constexpr (WN > 1) {
+      // the upper half of the groups into the lower half's registers, these into the buffer, and all warps from there
+      constexpr int HG = WN / 2;
+      block_sync();
+      if (grp >= HG) put((grp - HG) * WM + wm);
+      block_sync();
+      if (grp < HG) {
+        const float* const src = red + (grp * WM + wm) * 16 * S::kRedPitch;
+        const float* const ml = red_ml + (grp * WM + wm) * 32;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          const float* const at = src + (g + 8 * i) * S::kRedPitch;
           const float2 other = *reinterpret_cast<const float2*>(ml + 2 * (g + 8 * i));
           const float top = fmaxf(m[i], other.x);
           const float a = ex2_diff(m[i], top), b = ex2_diff(other.x, top);
           m[i] = top;
           l[i] = l[i] * a + other.y * b;
+          if constexpr (F8) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            o[n][2 * i] = o[n][2 * i] * a + src[(g + 8 * i) * S::kRedPitch + column(n, 0)] * b;
-            o[n][2 * i + 1] = o[n][2 * i + 1] * a + src[(g + 8 * i) * S::kRedPitch + column(n, 1)] * b;
-          }
-        }
-      }
-    }
-
-    const bool whole = cs.c0 == 0 && cs.c1 == cs.nch;
-    const float vs = F8 && p.kv.v_scale ? p.kv.v_scale[h] : 1.f;
-    const int slot = 2 * cta + (unit == u0 ? 0 : 1);
-    if (grp == 0) {
+            for (int n = 0; n < NT; n += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(at + n * 8 + 4 * t);
+              o[n][2 * i] = o[n][2 * i] * a + v.x * b;
+              o[n + 1][2 * i] = o[n + 1][2 * i] * a + v.y * b;
+              o[n][2 * i + 1] = o[n][2 * i + 1] * a + v.z * b;
+              o[n + 1][2 * i + 1] = o[n + 1][2 * i + 1] * a + v.w * b;
+            }
+          } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int rl = wm * 16 + g + 8 * i, r = tile0 + rl;
-        if (r >= p.rows) continue;
-        if (whole) {
-          const int tok = fdiv(r, p.group_div);
-          const int64_t at = ((int64_t)cs.b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
-          const float inv = l[i] == 0.f ? 0.f : vs / l[i];
-          T* dst = (T*)p.out + at * p.dim;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if constexpr (F8) {
-              if (n & 1) continue;
-              const int d = column(n, 0);
-              if (d < p.dim)
-                *reinterpret_cast<uint2*>(dst + d) =
-                    make_uint2(pack2<T>(o[n][2 * i] * inv, o[n + 1][2 * i] * inv),
-                               pack2<T>(o[n][2 * i + 1] * inv, o[n + 1][2 * i + 1] * inv));
-            } else {
-              const int d = column(n, 0);
-              if (d < p.dim)
-                *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+            for (int n = 0; n < NT; ++n) {
+              const float2 v = *reinterpret_cast<const float2*>(at + n * 8 + 2 * t);
+              o[n][2 * i] = o[n][2 * i] * a + v.x * b;
+              o[n][2 * i + 1] = o[n][2 * i + 1] * a + v.y * b;
             }
           }
-          if (p.lse && t == 0) p.lse[at] = l[i] == 0.f ? -INFINITY : m[i] * 0.6931471805599453f + logf(l[i]);
-        } else {
-          float* po = p.part_o + ((int64_t)slot * RT + rl) * DP;
-          if (t == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(m[i], l[i]);
+        }
+        __syncwarp();
+        put(grp * WM + wm);  // over what this warp alone has read
+      }
+      block_sync();
+      constexpr int V = DP / 4;  // threads of a row, four dimensions each
+      for (int x = tid; x < nrows * V; x += NW * 32) {
+        const int rl = x / V, d = (x - rl * V) * 4;
+        const int w0 = rl >> 4, rr = rl & 15;  // the warp of a group that had the row
+        float top = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if constexpr (F8) {
-              if (n & 1) continue;
-              *reinterpret_cast<float4*>(po + column(n, 0)) =
-                  make_float4(o[n][2 * i], o[n + 1][2 * i], o[n][2 * i + 1], o[n + 1][2 * i + 1]);
-            } else {
-              *reinterpret_cast<float2*>(po + column(n, 0)) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        for (int q = 0; q < HG; ++q) top = fmaxf(top, red_ml[(q * WM + w0) * 32 + 2 * rr]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < HG; ++q) {
+          const float2 ml = *reinterpret_cast<const float2*>(red_ml + (q * WM + w0) * 32 + 2 * rr);
+          const float4 v = *reinterpret_cast<const float4*>(red + ((q * WM + w0) * 16 + rr) * S::kRedPitch + d);
+          const float a = ex2_diff(ml.x, top);
+          sum += a * ml.y;
+          acc.x += a * v.x;
+          acc.y += a * v.y;
+          acc.z += a * v.z;
+          acc.w += a * v.w;
+        }
+        if (whole) {
+          const int64_t at = place(tile0 + rl);
+          const float inv = sum == 0.f ? 0.f : vs / sum;
+          if (d < p.dim)
+            *reinterpret_cast<uint2*>((T*)p.out + at * p.dim + d) =
+                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * RT + rl) * DP + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(top, sum);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rl = wm * 16 + g + 8 * i;
+        if (rl >= nrows) continue;
+        const int64_t at = place(tile0 + rl);
+        const float mul = !whole ? 1.f : l[i] == 0.f ? 0.f : vs / l[i];
+        T* const dst = (T*)p.out + at * p.dim;
+        float* const po = p.part_o + ((int64_t)slot * RT + rl) * DP;
+        if (t == 0) {
+          if (!whole)
+            *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(m[i], l[i]);
+          else if (p.lse)
+            p.lse[at] = l[i] == 0.f ? -INFINITY : m[i] * 0.6931471805599453f + logf(l[i]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          // two column tiles: dimensions 16 (n / 2) .. + 15
+          if constexpr (F8) {
+            const int d = n * 8 + 4 * t;
+            const float4 v = make_float4(o[n][2 * i] * mul, o[n + 1][2 * i] * mul, o[n][2 * i + 1] * mul, o[n + 1][2 * i + 1] * mul);
+            if (!whole)
+              *reinterpret_cast<float4*>(po + d) = v;
+            else if (d < p.dim)
+              *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = (n + e) * 8 + 2 * t;
+              const float x = o[n + e][2 * i] * mul, y = o[n + e][2 * i + 1] * mul;
+              if (!whole)
+                *reinterpret_cast<float2*>(po + d) = make_float2(x, y);
+              else if (d < p.dim)
+                *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(x, y);
             }
           }
         }
@@ -718,76 +667,21 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kWarps * 32, 1) attn_kernel(con
     }
     if (!whole) {
       // ---- the block that finishes a split (sequence, head) last joins its parts, in run order -----------------------
-      const int64_t a = unit - cs.c0, z = a + cs.nch;  // its chunks in the list of all
-      const int first = (int)(((a + 1) * blocks + total - 1) / total) - 1;
-      const int last = (int)((z * blocks + total - 1) / total) - 1;
+      const Split x = split_of(run, cs, unit);
       __threadfence();
-      __syncthreads();
-      if (tid == 0) s_last = atomicAdd(&p.counters[first], 1) == last - first;
-      __syncthreads();
+      block_sync();
+      if (tid == 0) s_last = atomicAdd(&p.counters[x.first], 1) == x.last - x.first;
+      block_sync();
       if (s_last) {
         __threadfence();
-        if (tid == 0) p.counters[first] = 0;
-        const int parts = last - first + 1;
-        // every block's part is that of its first chunk, but perhaps the first block's
-        const int first_slot = 2 * first + (first * total / blocks < a ? 1 : 0);
-        const auto slot_of = [&](int c) { return c == first ? first_slot : 2 * c; };
-        const int nrows = min(RT, p.rows - tile0);
-        constexpr int W = DP / 32;
-        for (int rl = warp; rl < nrows; rl += NW) {
-          float top = -INFINITY;
-          for (int q = lane; q < parts; q += 32)
-            top = fmaxf(top, __ldcg(p.part_ml + ((int64_t)slot_of(first + q) * RT + rl) * 2));
-#pragma unroll
-          for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-          float sum = 0.f, acc[W];
-#pragma unroll
-          for (int w = 0; w < W; ++w) acc[w] = 0.f;
-          for (int q0 = 0; q0 < parts; q0 += 32) {
-            float wt = 0.f;
-            if (q0 + lane < parts) {
-              const float2 ml =
-                  __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot_of(first + q0 + lane) * RT + rl) * 2));
-              wt = ex2_diff(ml.x, top);
-              sum += wt * ml.y;
-            }
-            const int n = min(32, parts - q0);
-#pragma unroll 8
-            for (int q = 0; q < n; ++q) {
-              const float wq = __shfl_sync(0xffffffffu, wt, q);
-              const float* src = p.part_o + ((int64_t)slot_of(first + q0 + q) * RT + rl) * DP + lane * W;
-              if constexpr (W == 2) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                acc[0] += wq * v.x;
-                acc[1] += wq * v.y;
-              } else {
-#pragma unroll
-                for (int w = 0; w < W; w += 4) {
-                  const float4 v = __ldcg(reinterpret_cast<const float4*>(src + w));
-                  acc[w] += wq * v.x;
-                  acc[w + 1] += wq * v.y;
-                  acc[w + 2] += wq * v.z;
-                  acc[w + 3] += wq * v.w;
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-          const int r = tile0 + rl, tok = fdiv(r, p.group_div);
-          const int64_t at = ((int64_t)cs.b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
-          const float inv = sum == 0.f ? 0.f : vs / sum;
-          T* dst = (T*)p.out + at * p.dim + lane * W;
-#pragma unroll
-          for (int w = 0; w < W; w += 2)
-            if (lane * W + w < p.dim) *reinterpret_cast<uint32_t*>(dst + w) = pack2<T>(acc[w] * inv, acc[w + 1] * inv);
-          if (p.lse && lane == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
-        }
+        if (tid == 0) p.counters[x.first] = 0;
+        join_parts<T, RT, DP>(p, x, cs.b, h, tile0, vs, warp, NW);
       }
     }
-    unit += cs.c1 - cs.c0;
-  } while (next_seg<CH, TOK>(p, cs));
-  cp_async_wait<0>();
+    if (!more) break;
+    unit += n_chunks;
+    cs = nx;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -795,7 +689,7 @@ int dim_class(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 // Warps that share a tile: enough for all rows of a kv head, so that its keys and values are read once.
 int row_warps(int rows, int dim) {
-  const int most = dim_class(dim) == 256 ? 4 : 8;
+  const int most = dim_class(dim) < 256 ? 8 : 4;
   int wm = 1;
   while (wm < most && 16 * wm < rows) wm *= 2;
   return wm;
@@ -826,7 +720,7 @@ int launch(const AttnParams& p, int sms, cudaStream_t stream) {
       return XCB_ERR_CUDA;
     if (dev < kMaxDevices) ready[dev] = true;
   }
-  attn_kernel<T, F8, DP, WM><<<sms, Shape<DP, F8>::kWarps * 32, bytes, stream>>>(p);
+  attn_kernel<T, F8, DP, WM><<<sms, Shape<DP, F8>::kThreads, bytes, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
 }
 template <typename T, bool F8, int DP>
@@ -910,6 +804,10 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   p.row_tiles = (p.rows + 16 * wm - 1) / (16 * wm);
   p.group_div = fast_div((uint32_t)p.group);
   p.head_div = fast_div((uint32_t)p.row_tiles);
+  // a row of a layer's keys has a 32-bit index, the list of chunks a 31-bit one
+  if ((int64_t)c->num_pages * c->kv_heads * c->page_size >= (1ll << 32) - 1 ||
+      (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1) >= 1ll << 31)
+    return XCB_ERR_UNSUPPORTED;
   const AttnWs w = attn_ws(sms, wm, dim_class(p.dim));
   if (ws_bytes < w.total) return XCB_ERR_WORKSPACE;
   p.counters = (int32_t*)((uint8_t*)ws + w.counters);
