@@ -33,6 +33,7 @@ namespace xcb {
 namespace {
 
 constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kSlack = 8.f;  // base 2, see attn_kernel's maximum
 
 // the rest of the 16 bytes is zeroed; with bytes = 0 nothing is read
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -72,7 +73,7 @@ __device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi)
 template <int DP, bool F8>
 struct Shape {
   static constexpr int kWarps = DP == 256 ? 4 : 8;   // consumers
-  static constexpr int kProducers = 2;
+  static constexpr int kProducers = 4;               // registers are given out by four warps: fewer would not free any
   static constexpr int kThreads = (kWarps + kProducers) * 32;
   static constexpr int kPitch = DP * (F8 ? 1 : 2);   // bytes of one position's row in shared memory
   static constexpr int kChunks = kPitch / 16;
@@ -88,7 +89,7 @@ struct Shape {
   static constexpr int kRedMl = kSlots * 16 * 2 * 4;
   static constexpr int kBars = 2 * kStages * 8;
   static constexpr int kMasks = kStages * (kCh / 32) * 4;
-  static constexpr int kScalars = 16 * 4;            // sums of the warps, then: place of the run's start, two flags
+  static constexpr int kScalars = 20 * 4;            // sums of the warps, then: place of the run's start, two flags
   static constexpr int kBytes = kRing + kRed + kRedMl + kBars + kMasks + kScalars;
 };
 
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
   constexpr int KS = DP / 16;       // 16-wide steps of the head dimension
   constexpr int NT = DP / 8;        // 8-wide column tiles of the output
   using M = typename std::conditional<F8, __half, T>::type;  // operand type of the tensor steps
-  static_assert(WM <= NW && CH % 64 == 0, "a group has at most the block's warps");
+  static_assert(WM <= NW && CH % 32 == 0, "a group has at most the block's warps");
 
   extern __shared__ __align__(1024) uint8_t smem[];  // all of the block's shared memory: stages start at multiples of 1 KB
   uint8_t* const ring = smem;
@@ -122,9 +123,9 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
   uint64_t* const empty = full + NS;
   uint32_t* const masks = reinterpret_cast<uint32_t*>(empty + NS);  // [NS][CH / 32]: positions that are there
   int* const s_sum = reinterpret_cast<int*>(masks + NS * (CH / 32));
-  int* const s_start = s_sum + 11;  // [3]
-  int& s_last = s_sum[14];
-  volatile int* const s_dead = s_sum + 15;
+  int* const s_start = s_sum + 12;  // [3]
+  int& s_last = s_sum[15];
+  volatile int* const s_dead = s_sum + 16;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -149,32 +150,31 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
   const int row_bytes = p.dim * (F8 ? 1 : 2);
 
   if (warp >= NW) {
-    // ---- producers: each warp half of every chunk's positions, 32 at a time -------------------------------------------
-    constexpr int UN = CH / 64, RPI = 32 / S::kChunks;
-    const int half = warp - NW;
+    // ---- producers: 32 positions at a time in turn -----------------------------------------------------------------------
+    constexpr int NP = S::kProducers, UN = (CH / 32 + NP - 1) / NP, RPI = 32 / S::kChunks;
+    const int me = warp - NW;
     const int lc = lane % S::kChunks, lr = lane / S::kChunks;  // this lane copies 16 bytes at lc of rows lr, lr + RPI, ..
     const int n_lane = lc * 16 < row_bytes ? 16 : 0;
     const uint8_t* const src0 = p.kv.k + (n_lane ? lc * 16 : 0);
     int ci = 0;
     bool more = true;
-    uint32_t next[UN];  // row of position `lane` of each 32 in the layer's keys, or ~0
+    // Of position `lane` of each 32 of the chunk to come: its page as read (-2: none wanted), and where in its page and
+    // head it lies.  Nothing is made of the page before its chunk's turn: the read is under way meanwhile.
+    int page[UN];
+    uint32_t within[UN];
     const auto look_up = [&]() {
 #pragma unroll
-      for (int u = 0; u < UN; ++u) next[u] = 0xffffffffu;
+      for (int u = 0; u < UN; ++u) page[u] = -2;
       if (!more) return;
-      const int pos0 = cs.t0 + ci * CH + half * (CH / 2) + lane;
       const int32_t* const row = p.kv.table + (int64_t)cs.row * p.kv.max_pages;
       const int h = fdiv(cs.j, p.head_div);
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
-        const int pos = pos0 + u * 32;
-        if (pos >= cs.lo && pos < cs.t1) {
+        const int at = (u * NP + me) * 32, pos = cs.t0 + ci * CH + at + lane;
+        if (at < CH && pos >= cs.lo && pos < cs.t1) {
           const int pi = fdiv(pos, p.kv.page_div);
-          const int page = row[pi];
-          if ((uint32_t)page < (uint32_t)p.kv.num_pages)
-            next[u] = ((uint32_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size);
-          else
-            atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
+          page[u] = row[pi];
+          within[u] = (uint32_t)h * p.kv.page_size + (pos - pi * p.kv.page_size);
         }
       }
       if (++ci == cs.c1 - cs.c0) {
@@ -182,20 +182,26 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         ci = 0;
       }
     };
+    const uint32_t page_rows = (uint32_t)p.kv.kv_heads * p.kv.page_size;
     look_up();
     int stage = 0;
     uint32_t parity = 1;  // the first round finds the stages empty
     for (int c = run.u0; c < run.u1; ++c) {
-      uint32_t cur[UN];
+      uint32_t cur[UN];  // row in the layer's keys, or ~0
 #pragma unroll
-      for (int u = 0; u < UN; ++u) cur[u] = next[u];
-      look_up();  // one chunk before it is needed
+      for (int u = 0; u < UN; ++u) {
+        const bool there = (uint32_t)page[u] < (uint32_t)p.kv.num_pages;
+        if (!there && page[u] != -2) atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
+        cur[u] = there ? (uint32_t)page[u] * page_rows + within[u] : 0xffffffffu;
+      }
+      look_up();
       wait(empty + stage, parity);
       if (!*s_dead) {
         const uint32_t dst0 = smem_u32(ring) + stage * (2 * S::kHalf);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-          const int r0 = half * (CH / 2) + u * 32;
+          const int r0 = (u * NP + me) * 32;
+          if (r0 >= CH) break;
           const uint32_t mask = __ballot_sync(0xffffffffu, cur[u] != 0xffffffffu);
           if (lane == 0) masks[stage * (CH / 32) + r0 / 32] = mask;
 #pragma unroll 8
@@ -391,7 +397,9 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * to_log2[i];
         }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+        // A lazy maximum: exponentials are taken against a reference that moves only when a score exceeds it by kSlack,
+        // so the sums are rarely rescaled; up to 2^8 too large, they lose nothing in 32 bits, nor do the operands.
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
           float a[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
