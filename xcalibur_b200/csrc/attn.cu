@@ -11,10 +11,11 @@
 // Split: the work is cut into chunks of 16 * warps positions and the list of all chunks (sequence by sequence, head
 // by head) into as many equal runs as there are SMs, found on the device from the lengths, so that ragged batches and
 // single long sequences keep every SM busy alike and nothing waits for the host.  A (sequence, head) that lies in
-// several runs is joined by the block that finishes it last, in run order whoever that is, so results do not depend on
-// timing.
+// several runs is joined by a second, small kernel, in run order, so results do not depend on timing; it is launched
+// along with the first and waits for it on the device.  (Joined by whichever block came last instead, 37 parts of
+// 131072 positions took one SM 7 us behind all others, and every part a fence and an atomic, 1 to 2 us.)
 //
-// Inside a block two producer warps copy chunk after chunk into a ring of shared-memory stages (cp.async, 16 bytes a
+// Inside a block four producer warps copy chunk after chunk into a ring of shared-memory stages (cp.async, 16 bytes a
 // lane, swizzled so that ldmatrix has no bank conflicts, positions that are not there as zeros) and run ahead over the
 // ends of segments; up to eight consumer warps compute.  Consumers are WN groups of WM warps: a group takes its share
 // of a chunk's positions, the warps of a group 16 rows each (WM = 1, 2, 4, 8 for up to 128 rows).  Stages pass between
@@ -104,7 +105,8 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {  // when this t
 }
 
 template <typename T, bool F8, int DP, int WM>
-__global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const __grid_constant__ AttnParams p) {
+  pdl_launch_dependents();
   using S = Shape<DP, F8>;
   constexpr int NW = S::kWarps, WN = NW / WM, NS = S::kStages;
   constexpr int TOK = S::kTok, SN = TOK / 8;
@@ -124,7 +126,6 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
   uint32_t* const masks = reinterpret_cast<uint32_t*>(empty + NS);  // [NS][CH / 32]: positions that are there
   int* const s_sum = reinterpret_cast<int*>(masks + NS * (CH / 32));
   int* const s_start = s_sum + 12;  // [3]
-  int& s_last = s_sum[15];
   volatile int* const s_dead = s_sum + 16;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -137,16 +138,19 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     *s_dead = 0;
   }
   Run run;
-  if (!plan_run<CH>(p, TOK, s_sum, s_start, run)) return;  // two block barriers: the set-up above is visible
+  Seg cs;
+  int u_seg;  // the unit of its first segment that the run starts with
+  const bool work = plan_run<CH, S::kThreads / 32>(p, TOK, s_sum, s_start, run, cs, &u_seg) &&
+                    open_seg<CH>(p, cs, u_seg, run.u1 - run.u0, TOK);
+  if (!work) {  // no units, or lead units alone
+    if (tid == 0) p.splits[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
 
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!*s_dead && !mbar_wait(bar, parity, kWaitNs, p.kv.status)) *s_dead = 1;
     __syncwarp();
   };
-  Seg cs;
-  cs.b = s_start[0];
-  cs.j = s_start[1];
-  open_seg<CH>(p, cs, s_start[2], run.u1 - run.u0, TOK);
   const int row_bytes = p.dim * (F8 ? 1 : 2);
 
   if (warp >= NW) {
@@ -165,7 +169,6 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     const auto look_up = [&]() {
 #pragma unroll
       for (int u = 0; u < UN; ++u) page[u] = -2;
-      if (!more) return;
       const int32_t* const row = p.kv.table + (int64_t)cs.row * p.kv.max_pages;
       const int h = fdiv(cs.j, p.head_div);
 #pragma unroll
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     look_up();
     int stage = 0;
     uint32_t parity = 1;  // the first round finds the stages empty
-    for (int c = run.u0; c < run.u1; ++c) {
+    for (;;) {
       uint32_t cur[UN];  // row in the layer's keys, or ~0
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
@@ -194,7 +197,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         if (!there && page[u] != -2) atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
         cur[u] = there ? (uint32_t)page[u] * page_rows + within[u] : 0xffffffffu;
       }
-      look_up();
+      const bool again = more;
+      if (again) look_up();
       wait(empty + stage, parity);
       if (!*s_dead) {
         const uint32_t dst0 = smem_u32(ring) + stage * (2 * S::kHalf);
@@ -219,6 +223,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
       cp_async_arrive(full + stage);
       __syncwarp();
       if (lane == 0) mbar_arrive(full + stage);
+      if (!again) break;
       if (++stage == NS) {
         stage = 0;
         parity ^= 1;
@@ -269,7 +274,9 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
 
   int stage = 0;
   uint32_t parity = 0;
-  int unit = run.u0;  // first chunk of the current segment
+  int unit = run.u0 - u_seg + kLead + cs.c0;  // the list's index of the segment's first chunk here
+  int part_slot = 2 * cta;
+  int4 split = make_int4(-1, 0, 0, 0);
   for (;;) {
     const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
     // positions that this lane's two rows see
@@ -527,7 +534,6 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     }
     Seg nx = cs;
     const bool more = next_seg<CH>(p, nx, TOK);
-    if (more) load_q(nx);  // under way while the parts are joined
 
     // ---- join the block's groups and write -----------------------------------------------------------------------------
 #pragma unroll
@@ -537,7 +543,6 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     }
     const bool whole = cs.c0 == 0 && cs.c1 == cs.nch;
     const float vs = F8 && p.kv.v_scale ? p.kv.v_scale[h] : 1.f;
-    const int slot = 2 * cta + (unit == run.u0 ? 0 : 1);
     const int nrows = min(RT, p.rows - tile0);
     const auto place = [&](int r) {  // of row r of the kv head in the output
       const int tok = fdiv(r, p.group_div);
@@ -601,6 +606,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         __syncwarp();
         put(grp * WM + wm);  // over what this warp alone has read
       }
+      if (more) load_q(nx);  // under way while the parts are joined
       block_sync();
       constexpr int V = DP / 4;  // threads of a row, four dimensions each
       for (int x = tid; x < nrows * V; x += NW * 32) {
@@ -630,8 +636,8 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
                 make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
           if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
         } else {
-          *reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * RT + rl) * DP + d) = acc;
-          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(top, sum);
+          *reinterpret_cast<float4*>(p.part_o + ((int64_t)part_slot * RT + rl) * DP + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)part_slot * RT + rl) * 2) = make_float2(top, sum);
         }
       }
     } else {
@@ -642,10 +648,10 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         const int64_t at = place(tile0 + rl);
         const float mul = !whole ? 1.f : l[i] == 0.f ? 0.f : vs / l[i];
         T* const dst = (T*)p.out + at * p.dim;
-        float* const po = p.part_o + ((int64_t)slot * RT + rl) * DP;
+        float* const po = p.part_o + ((int64_t)part_slot * RT + rl) * DP;
         if (t == 0) {
           if (!whole)
-            *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * RT + rl) * 2) = make_float2(m[i], l[i]);
+            *reinterpret_cast<float2*>(p.part_ml + ((int64_t)part_slot * RT + rl) * 2) = make_float2(m[i], l[i]);
           else if (p.lse)
             p.lse[at] = l[i] == 0.f ? -INFINITY : m[i] * 0.6931471805599453f + logf(l[i]);
         }
@@ -673,22 +679,88 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         }
       }
     }
-    if (!whole) {
-      // ---- the block that finishes a split (sequence, head) last joins its parts, in run order -----------------------
-      const Split x = split_of(run, cs, unit);
-      __threadfence();
-      block_sync();
-      if (tid == 0) s_last = atomicAdd(&p.counters[x.first], 1) == x.last - x.first;
-      block_sync();
-      if (s_last) {
-        __threadfence();
-        if (tid == 0) p.counters[x.first] = 0;
-        join_parts<T, RT, DP>(p, x, cs.b, h, tile0, vs, warp, NW);
+    if (WN == 1 && more) load_q(nx);
+    if (!whole && cs.c0 == 0) split = split_of(run, cs, unit, part_slot);
+    if (!more) break;
+    unit += cs.nch - cs.c0 + kLead;
+    part_slot = 2 * cta + 1;
+    cs = nx;
+  }
+  if (tid == 0) p.splits[cta] = split;
+}
+
+// Joins the parts of the split segment that block blockIdx.x of attn_kernel began, if it did: a warp takes a row at a
+// time, a lane DP / 32 dimensions, parts in run order.  Bound: latency, two or three rounds of reads.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams p, int rt) {
+  constexpr int W = DP / 32, U = 64 / W;  // parts whose rows are read at once
+  pdl_wait();
+  const int4 sp = p.splits[blockIdx.x];
+  if (sp.x < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = blockIdx.x, parts = sp.z - first + 1;
+  const int h = fdiv(sp.y, p.head_div), tile0 = (sp.y - h * p.row_tiles) * rt;
+  const int nrows = min(rt, p.rows - tile0);
+  const float vs = p.kv.v_scale ? p.kv.v_scale[h] : 1.f;
+  const auto slot_of = [&](int i) { return i == 0 ? sp.w : 2 * (first + i); };
+  for (int rl = blockIdx.y * 8 + warp; rl < nrows; rl += gridDim.y * 8) {
+    float top = -INFINITY, sum = 0.f, acc[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) acc[w] = 0.f;
+    const float* const row_ml = p.part_ml + rl * 2;
+    const float* const row_o = p.part_o + (int64_t)rl * DP + lane * W;
+    for (int q0 = 0; q0 < parts; q0 += 32) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (q0 + lane < parts) ml = *reinterpret_cast<const float2*>(row_ml + (int64_t)slot_of(q0 + lane) * rt * 2);
+      const int n = min(32, parts - q0);
+      float wt = 0.f;
+      for (int q = 0; q < n; q += U) {
+        float v[U][W];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (q + u < n) {
+            const float* const src = row_o + (int64_t)slot_of(q0 + q + u) * rt * DP;
+            if constexpr (W == 2) {
+              *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src);
+            } else {
+#pragma unroll
+              for (int w = 0; w < W; w += 4)
+                *reinterpret_cast<float4*>(v[u] + w) = *reinterpret_cast<const float4*>(src + w);
+            }
+          }
+        }
+        if (q == 0) {  // the maxima of these 32 parts; what came before is scaled to the new one
+          float now = ml.x;
+#pragma unroll
+          for (int s = 16; s; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+          now = fmaxf(now, top);
+          const float scale = ex2_diff(top, now);
+          wt = ex2_diff(ml.x, now);
+          top = now;
+          sum = sum * scale + wt * ml.y;
+#pragma unroll
+          for (int w = 0; w < W; ++w) acc[w] *= scale;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float wq = __shfl_sync(0xffffffffu, wt, (q + u) & 31);
+          if (q + u < n) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) acc[w] += wq * v[u][w];
+          }
+        }
       }
     }
-    if (!more) break;
-    unit += n_chunks;
-    cs = nx;
+#pragma unroll
+    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const int r = tile0 + rl, tok = fdiv(r, p.group_div);
+    const int64_t at = ((int64_t)sp.x * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
+    const float inv = sum == 0.f ? 0.f : vs / sum;
+    T* const dst = (T*)p.out + at * p.dim + lane * W;
+#pragma unroll
+    for (int w = 0; w < W; w += 2)
+      if (lane * W + w < p.dim) *reinterpret_cast<uint32_t*>(dst + w) = pack2<T>(acc[w] * inv, acc[w + 1] * inv);
+    if (p.lse && lane == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
   }
 }
 
@@ -704,12 +776,12 @@ int row_warps(int rows, int dim) {
 }
 
 struct AttnWs {
-  size_t counters, ml, o, total;
+  size_t splits, ml, o, total;
 };
 AttnWs attn_ws(int sms, int wm, int dp) {
   AttnWs w;
-  w.counters = 0;
-  w.ml = ((size_t)sms * 4 + 255) / 256 * 256;
+  w.splits = 0;
+  w.ml = ((size_t)sms * 16 + 255) / 256 * 256;
   w.o = w.ml + ((size_t)2 * sms * 16 * wm * 8 + 255) / 256 * 256;
   w.total = w.o + (size_t)2 * sms * 16 * wm * dp * 4;
   return w;
@@ -729,7 +801,19 @@ int launch(const AttnParams& p, int sms, cudaStream_t stream) {
     if (dev < kMaxDevices) ready[dev] = true;
   }
   attn_kernel<T, F8, DP, WM><<<sms, Shape<DP, F8>::kThreads, bytes, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return XCB_ERR_CUDA;
+  // the join is launched along with it and waits on the device for its end
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  const int rt = 16 * WM;
+  cfg.gridDim = dim3(sms, (unsigned)((p.rows < rt ? p.rows : rt) + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<T, DP>, p, rt) == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
 }
 template <typename T, bool F8, int DP>
 int launch_wm(const AttnParams& p, int wm, int sms, cudaStream_t stream) {
@@ -814,11 +898,11 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   p.head_div = fast_div((uint32_t)p.row_tiles);
   // a row of a layer's keys has a 32-bit index, the list of chunks a 31-bit one
   if ((int64_t)c->num_pages * c->kv_heads * c->page_size >= (1ll << 32) - 1 ||
-      (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1) >= 1ll << 31)
+      (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1 + kLead) >= 1ll << 31)
     return XCB_ERR_UNSUPPORTED;
   const AttnWs w = attn_ws(sms, wm, dim_class(p.dim));
   if (ws_bytes < w.total) return XCB_ERR_WORKSPACE;
-  p.counters = (int32_t*)((uint8_t*)ws + w.counters);
+  p.splits = (int4*)((uint8_t*)ws + w.splits);
   p.part_ml = (float*)((uint8_t*)ws + w.ml);
   p.part_o = (float*)((uint8_t*)ws + w.o);
   if (c->dtype == XCB_DTYPE_E4M3)

@@ -1,5 +1,5 @@
-// Paged attention: a call's parameters, the split of the work over the blocks, and the join of a (sequence, head) that
-// several blocks worked on.
+// Paged attention: a call's parameters, the split of the work over the blocks, and the record of a (sequence,
+// head) that several blocks worked on.
 #pragma once
 #include <math.h>
 
@@ -18,7 +18,7 @@ struct AttnParams {
   int32_t batch, new_tokens, group, q_heads, rows, row_tiles, dim, window;
   float scale_log2;
   FastDiv group_div, head_div;  // head_div: by row_tiles
-  int32_t* counters;            // [blocks], zero between calls
+  int4* splits;                 // [blocks] the split segment whose first part a block holds (x < 0: none)
   float* part_ml;               // [2 * blocks][rows of a tile][2]
   float* part_o;                // [2 * blocks][rows of a tile][padded head_dim]
 };
@@ -31,12 +31,17 @@ __device__ __forceinline__ float ex2(float x) {
 // e^(a - b) in base 2 where b is a maximum that may be -inf (nothing seen yet)
 __device__ __forceinline__ float ex2_diff(float a, float b) { return ex2(a - (b == -INFINITY ? 0.f : b)); }
 
+// The work is a list of units: for every (sequence, kv head, row tile) kLead units that stand for the cost of its
+// start and end (queries, join, write: about a chunk's time, measured 1 to 1.5 us against 1.5 us for 64 KB), then its
+// chunks of CH positions.  Blocks get equal runs of units; one that gets lead units alone has nothing to do there.
+constexpr int kLead = 1;
+
 // A run of chunks of one (sequence, kv head, row tile).
 struct Seg {
   int b, j, row;        // sequence of the batch; head * row_tiles + tile; row of the page table
   int len, c0, c1, nch; // visible end; chunks [c0, c1) of nch
   int t0, t1, lo;       // positions of these chunks; the first that any row sees
-  int left;             // chunks of the block's run after this segment
+  int left;             // units of the block's run after this segment
 };
 
 __device__ __forceinline__ int visible(const AttnParams& p, int b, int* row, int* lo) {
@@ -56,15 +61,17 @@ template <int CH>
 __device__ __forceinline__ int chunks_of(int len, int lo, int align) {
   return max(1, (len - (lo & -align) + CH - 1) / CH);  // an empty sequence is one empty chunk: its rows are written too
 }
+// The segment of s.b, s.j from its unit u0 on, with `units` units left.  False: lead units alone were left.
 template <int CH>
-__device__ __forceinline__ void open_seg(const AttnParams& p, Seg& s, int c0, int units, int align) {
+__device__ __forceinline__ bool open_seg(const AttnParams& p, Seg& s, int u0, int units, int align) {
   s.len = visible(p, s.b, &s.row, &s.lo);
   s.nch = chunks_of<CH>(s.len, s.lo, align);
-  s.c0 = c0;
-  s.c1 = min(s.nch, c0 + units);
-  s.left = units - (s.c1 - s.c0);
-  s.t0 = (s.lo & -align) + c0 * CH;
+  s.c0 = max(0, u0 - kLead);
+  s.c1 = min(s.nch, u0 + units - kLead);
+  s.left = u0 + units - (s.nch + kLead);
+  s.t0 = (s.lo & -align) + s.c0 * CH;
   s.t1 = min(s.len, (s.lo & -align) + s.c1 * CH);
+  return s.c1 > s.c0;
 }
 template <int CH>
 __device__ __forceinline__ bool next_seg(const AttnParams& p, Seg& s, int align) {
@@ -73,14 +80,13 @@ __device__ __forceinline__ bool next_seg(const AttnParams& p, Seg& s, int align)
     s.j = 0;
     if (++s.b >= p.batch) return false;
   }
-  open_seg<CH>(p, s, 0, s.left, align);
-  return true;
+  return open_seg<CH>(p, s, 0, s.left, align);
 }
 
-// The list of all chunks (sequence by sequence, head by head) in `blocks` runs whose lengths differ by one at most:
-// block c's is [start(c), start(c + 1)).  Counts fit 31 bits (checked on the host).
+// The units in `blocks` runs whose lengths differ by one at most: block c's is [start(c), start(c + 1)).  Counts fit 31
+// bits (checked on the host).
 struct Run {
-  int blocks, each, longer;  // the first `longer` blocks have each + 1 chunks
+  int blocks, each, longer;  // the first `longer` blocks have each + 1 units
   int u0, u1;                // this block's
   __device__ __forceinline__ int start(int c) const { return c * each + min(c, longer); }
   __device__ __forceinline__ int owner(int u) const {
@@ -88,20 +94,25 @@ struct Run {
     return u < edge ? u / (each + 1) : longer + (u - edge) / each;
   }
 };
-// All threads of the block (a multiple of 32, at most 1024).  s_sum: one value per warp; s_start: the place of u0.
-// False: the block has no run.
-template <int CH>
-__device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_sum, int* s_start, Run& run) {
+// All threads of the block of WARPS warps.  s_sum: one value per warp.  Puts the place of the run's start (sequence,
+// head and row tile, unit of the segment) into s.b, s.j, *unit.  False: the block has no run.  The block meets at a
+// barrier at least once.
+template <int CH, int WARPS>
+__device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_sum, int* s_start, Run& run, Seg& s,
+                                         int* unit) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const int heads = p.kv.kv_heads * p.row_tiles;
-  const int per = (p.batch + blockDim.x - 1) / blockDim.x;
-  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  int mine = 0;
+  const bool small = p.batch <= 32;  // every warp plans for itself
+  const int me = small ? lane : tid;
+  const int per = small ? 1 : (p.batch + WARPS * 32 - 1) / (WARPS * 32);
+  const int b0 = min(p.batch, me * per), b1 = min(p.batch, b0 + per);
+  int mine = 0, units0 = 0;
   for (int b = b0; b < b1; ++b) {
     int row, lo;
     const int len = visible(p, b, &row, &lo);
-    mine += chunks_of<CH>(len, lo, align) * heads;
-    if (cta == 0 && (row < 0 || row >= p.kv.max_seqs)) atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
+    units0 = kLead + chunks_of<CH>(len, lo, align);
+    mine += units0 * heads;
+    if (cta == 0 && warp == (small ? 0 : warp) && (row < 0 || row >= p.kv.max_seqs)) atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
   }
   int incl = mine;
 #pragma unroll
@@ -109,13 +120,19 @@ __device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-    const int v = s_sum[w];
-    if (w < warp) before += v;
-    all += v;
+  int before = 0, all;
+  if (small) {
+    all = __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const int v = s_sum[w];
+      if (w < warp) before += v;
+      all += v;
+    }
   }
   run.blocks = min((int)gridDim.x, all);
   if (cta >= run.blocks) return false;
@@ -124,94 +141,43 @@ __device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_
   run.u0 = run.start(cta);
   run.u1 = run.start(cta + 1);
   int at = before + incl - mine;
-  if (run.u0 >= at && run.u0 < at + mine) {
-    for (int b = b0; b < b1; ++b) {
-      int row, lo;
-      const int len = visible(p, b, &row, &lo);
-      const int nch = chunks_of<CH>(len, lo, align);
-      if (run.u0 < at + nch * heads) {
-        s_start[0] = b;
-        s_start[1] = (run.u0 - at) / nch;
-        s_start[2] = (run.u0 - at) % nch;
-        break;
+  const bool found = run.u0 >= at && run.u0 < at + mine;
+  int place[3] = {0, 0, 0};
+  if (found) {
+    int b = b0;
+    if (per > 1) {
+      for (;; ++b) {
+        int row, lo;
+        const int len = visible(p, b, &row, &lo);
+        units0 = kLead + chunks_of<CH>(len, lo, align);
+        if (b == b1 - 1 || run.u0 < at + units0 * heads) break;
+        at += units0 * heads;
       }
-      at += nch * heads;
     }
+    place[0] = b;
+    place[1] = (run.u0 - at) / units0;
+    place[2] = (run.u0 - at) - place[1] * units0;
+    if (!small) s_start[0] = place[0], s_start[1] = place[1], s_start[2] = place[2];
   }
   __syncthreads();
+  if (small) {
+    const int who = __ffs(__ballot_sync(0xffffffffu, found)) - 1;
+    s.b = __shfl_sync(0xffffffffu, place[0], who);
+    s.j = __shfl_sync(0xffffffffu, place[1], who);
+    *unit = __shfl_sync(0xffffffffu, place[2], who);
+  } else {
+    s.b = s_start[0];
+    s.j = s_start[1];
+    *unit = s_start[2];
+  }
   return true;
 }
 
-// Which blocks share a segment: those that own its first and its last chunk, and all between.
-struct Split {
-  int first, last, first_slot;
-};
-__device__ __forceinline__ Split split_of(const Run& r, const Seg& s, int unit) {
-  const int a = unit - s.c0;  // its chunks in the list of all: a .. a + nch - 1
-  Split x;
-  x.first = r.owner(a);
-  x.last = r.owner(a + s.nch - 1);
-  // every block's part is that of its first chunk, but perhaps the first block's
-  x.first_slot = 2 * x.first + (r.start(x.first) < a ? 1 : 0);
-  return x;
-}
-
-// Warps `warp` of `warps` join the parts of a segment's rows in run order and write them out.
-template <typename T, int RT, int DP>
-__device__ __forceinline__ void join_parts(const AttnParams& p, const Split& x, int b, int h, int tile0, float vs,
-                                           int warp, int warps) {
-  constexpr int W = DP / 32;
-  const int lane = threadIdx.x & 31;
-  const int parts = x.last - x.first + 1;
-  const int nrows = min(RT, p.rows - tile0);
-  const auto slot_of = [&](int i) { return i == 0 ? x.first_slot : 2 * (x.first + i); };
-  for (int rl = warp; rl < nrows; rl += warps) {
-    float top = -INFINITY;
-    for (int q = lane; q < parts; q += 32) top = fmaxf(top, __ldcg(p.part_ml + ((int64_t)slot_of(q) * RT + rl) * 2));
-#pragma unroll
-    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    float sum = 0.f, acc[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) acc[w] = 0.f;
-    for (int q0 = 0; q0 < parts; q0 += 32) {
-      float wt = 0.f;
-      if (q0 + lane < parts) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((int64_t)slot_of(q0 + lane) * RT + rl) * 2));
-        wt = ex2_diff(ml.x, top);
-        sum += wt * ml.y;
-      }
-      const int n = min(32, parts - q0);
-#pragma unroll 8
-      for (int q = 0; q < n; ++q) {
-        const float wq = __shfl_sync(0xffffffffu, wt, q);
-        const float* src = p.part_o + ((int64_t)slot_of(q0 + q) * RT + rl) * DP + lane * W;
-        if constexpr (W == 2) {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] += wq * v.x;
-          acc[1] += wq * v.y;
-        } else {
-#pragma unroll
-          for (int w = 0; w < W; w += 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + w));
-            acc[w] += wq * v.x;
-            acc[w + 1] += wq * v.y;
-            acc[w + 2] += wq * v.z;
-            acc[w + 3] += wq * v.w;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    const int r = tile0 + rl, tok = fdiv(r, p.group_div);
-    const int64_t at = ((int64_t)b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
-    const float inv = sum == 0.f ? 0.f : vs / sum;
-    T* dst = (T*)p.out + at * p.dim + lane * W;
-#pragma unroll
-    for (int w = 0; w < W; w += 2)
-      if (lane * W + w < p.dim) *reinterpret_cast<uint32_t*>(dst + w) = pack2<T>(acc[w] * inv, acc[w + 1] * inv);
-    if (p.lse && lane == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
-  }
+// A split segment's first block records it for the join: sequence, head and row tile, last block, slot of its part.  A
+// block's part lies in the first of its two slots if the segment is the first that it works on, as it is for every
+// block but perhaps the first.  `unit`: the list's index of the segment's chunk 0.
+__device__ __forceinline__ int4 split_of(const Run& r, const Seg& s, int unit, int slot) {
+  return make_int4(s.b, s.j, r.owner(unit + s.nch - 1), slot);
 }
 
 }  // namespace xcb
