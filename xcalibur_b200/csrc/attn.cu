@@ -270,36 +270,16 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
       }
     }
   };
-  load_q(cs);
-
-  int stage = 0;
-  uint32_t parity = 0;
-  int unit = run.u0 - u_seg + kLead + cs.c0;  // the list's index of the segment's first chunk here
-  int part_slot = 2 * cta;
-  int4 split = make_int4(-1, 0, 0, 0);
-  for (;;) {
-    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
-    // positions that this lane's two rows see
-    int hi[2], lo[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = tile0 + wm * 16 + g + 8 * i;
-      hi[i] = cs.len;
-      lo[i] = 0;
-      if (p.new_tokens > 1 && r < p.rows) {
-        hi[i] = cs.len - p.new_tokens + fdiv(r, p.group_div) + 1;
-        lo[i] = p.window ? max(0, hi[i] - p.window) : 0;
-      }
-    }
-    float to_log2[2];
+  // Operands of the tensor steps from the rows, and the factors of their scores.
+  const auto make_q = [&](int h, float (&to_log2)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       to_log2[i] = p.scale_log2;
       if constexpr (F8) {
         if (p.kv.k_scale) to_log2[i] *= p.kv.k_scale[h];
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          // bf16 queries as f16: scaled by a power of two that brings the row's largest value to [2^14, 2^15), which
-          // is exact down to 2^-38 of that value
+          // bf16 queries as f16: scaled by a power of two that brings the row's largest value to [2^14, 2^15), exact
+          // down to 2^-38 of that value.
           float top = 0.f;
 #pragma unroll
           for (int kk = 0; kk < KS; ++kk) {
@@ -309,7 +289,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const int ex = (int)(__float_as_uint(top) >> 23);                // biased exponent, 255: not finite
-          const int up = ex == 255 || ex == 0 ? 0 : max(-100, min(100, 127 + 14 - ex));
+          const int up = ex == 0 || ex == 255 ? 0 : max(-120, min(120, 127 + 14 - ex));
           const float mul = __uint_as_float((uint32_t)(127 + up) << 23), inv = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
           for (int kk = 0; kk < KS; ++kk) {
@@ -334,6 +314,55 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
       }
       to_log2[i] = fmaxf(to_log2[i], 1e-37f);
     }
+  };
+  // With an 8-bit cache the operands stay in shared memory, in the lanes' order, for all groups (in the join's buffer,
+  // which is free between joins): the registers are needed for the keys' and values' conversions.
+  uint4* const q_frag = reinterpret_cast<uint4*>(red);  // [WM][KS][32]
+  static_assert(!F8 || WM * KS * 512 <= S::kRed, "the join's buffer holds the queries");
+  if (!F8 || grp == 0) load_q(cs);
+
+  int stage = 0;
+  uint32_t parity = 0;
+  int unit = run.u0 - u_seg + kLead + cs.c0;  // the list's index of the segment's first chunk here
+  int part_slot = 2 * cta;
+  int4 split = make_int4(-1, 0, 0, 0);
+  for (;;) {
+    const int h = fdiv(cs.j, p.head_div), tile0 = (cs.j - h * p.row_tiles) * RT;
+    // positions that this lane's two rows see
+    int hi[2], lo[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = tile0 + wm * 16 + g + 8 * i;
+      hi[i] = cs.len;
+      lo[i] = 0;
+      if (p.new_tokens > 1 && r < p.rows) {
+        hi[i] = cs.len - p.new_tokens + fdiv(r, p.group_div) + 1;
+        lo[i] = p.window ? max(0, hi[i] - p.window) : 0;
+      }
+    }
+    float to_log2[2];
+    if constexpr (F8) {
+      if constexpr (WN > 1) block_sync();  // the join has been read
+      if (grp == 0) {
+        make_q(h, to_log2);
+        uint4* const dst = q_frag + wm * KS * 32 + lane;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) dst[kk * 32] = make_uint4(qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+        if (t == 0) {
+          red_ml[wm * 16 + g] = to_log2[0];
+          red_ml[wm * 16 + g + 8] = to_log2[1];
+        }
+      }
+      if constexpr (WN > 1) {
+        block_sync();
+        to_log2[0] = red_ml[wm * 16 + g];
+        to_log2[1] = red_ml[wm * 16 + g + 8];
+      } else {
+        __syncwarp();
+      }
+    } else {
+      make_q(h, to_log2);
+    }
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -354,25 +383,30 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         float s[SN][4];
 #pragma unroll
         for (int n = 0; n < SN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        // the swizzle again: chunk 2 kk + cc of the lane's row is the lane's address xor 32 kk
+        if constexpr (F8) {
+          const uint4* const q_lane = q_frag + wm * KS * 32 + lane;
 #pragma unroll
-        for (int b = 0; b < SN / 2; ++b) {
-          // the swizzle again: chunk 2 kk + cc of the lane's row is the lane's address xor 32 kk
-          const uint32_t ka = kb + k_lane + b * 16 * S::kPitch;
-          if constexpr (F8) {
+          for (int k2 = 0; k2 < KS / 2; ++k2) {
+            const uint4 qa = q_lane[2 * k2 * 32], qb = q_lane[(2 * k2 + 1) * 32];
 #pragma unroll
-            for (int k2 = 0; k2 < KS / 2; ++k2) {
+            for (int b = 0; b < SN / 2; ++b) {
               uint32_t w[4];
-              ldsm4(w, ka ^ (k2 << 5));
+              ldsm4(w, (kb + k_lane + b * 16 * S::kPitch) ^ (k2 << 5));
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
+              for (int n = 0; n < 2; ++n) {
                   uint32_t b0, b1;
-                  e4m3_f16(w[2 * n + e], b0, b1);
-                  mma16<M>(s[2 * b + n], qf[2 * k2 + e], b0, b1);
-                }
+                  e4m3_f16(w[2 * n], b0, b1);
+                  mma16<M>(s[2 * b + n], {qa.x, qa.y, qa.z, qa.w}, b0, b1);
+                  e4m3_f16(w[2 * n + 1], b0, b1);
+                  mma16<M>(s[2 * b + n], {qb.x, qb.y, qb.z, qb.w}, b0, b1);
+              }
             }
-          } else {
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < SN / 2; ++b) {
+            const uint32_t ka = kb + k_lane + b * 16 * S::kPitch;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
               uint32_t w[4];
@@ -606,7 +640,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
         __syncwarp();
         put(grp * WM + wm);  // over what this warp alone has read
       }
-      if (more) load_q(nx);  // under way while the parts are joined
+      if (more && (!F8 || grp == 0)) load_q(nx);  // under way while the parts are joined
       block_sync();
       constexpr int V = DP / 4;  // threads of a row, four dimensions each
       for (int x = tid; x < nrows * V; x += NW * 32) {
