@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
 
   int stage = 0;
   uint32_t parity = 0;
-  int unit = run.u0 - u_seg + kLead + cs.c0;  // the list's index of the segment's first chunk here
+  int unit = run.u0 - u_seg + p.lead + cs.c0;  // the list's index of the segment's first chunk here
   int part_slot = 2 * cta;
   int4 split = make_int4(-1, 0, 0, 0);
   for (;;) {
@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
     if (WN == 1 && more) load_q(nx);
     if (!whole && cs.c0 == 0) split = split_of(run, cs, unit, part_slot);
     if (!more) break;
-    unit += cs.nch - cs.c0 + kLead;
+    unit += cs.nch - cs.c0 + p.lead;
     part_slot = 2 * cta + 1;
     cs = nx;
   }
@@ -928,11 +928,15 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const int wm = row_warps(p.rows, p.dim);
   p.row_tiles = (p.rows + 16 * wm - 1) / (16 * wm);
+  // What a segment's ends cost in chunks.  64 ragged sequences, 8 rows: 52.4 / 48.9 / 49.9 us with 1 / 2 / 3; 8 bits, 128
+  // sequences, 8 rows: 102.7 / 85.4 / 87.4.  With more rows a chunk itself costs more: 4 draft tokens of 48 sequences, 20
+  // rows: 59.0 / 60.5 / 63.1.
+  p.lead = p.rows <= 16 ? 2 : 1;
   p.group_div = fast_div((uint32_t)p.group);
   p.head_div = fast_div((uint32_t)p.row_tiles);
   // a row of a layer's keys has a 32-bit index, the list of chunks a 31-bit one
   if ((int64_t)c->num_pages * c->kv_heads * c->page_size >= (1ll << 32) - 1 ||
-      (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1 + kLead) >= 1ll << 31)
+      (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1 + p.lead) >= 1ll << 31)
     return XCB_ERR_UNSUPPORTED;
   const AttnWs w = attn_ws(sms, wm, dim_class(p.dim));
   if (ws_bytes < w.total) return XCB_ERR_WORKSPACE;

@@ -15,7 +15,7 @@ struct AttnParams {
   void* out;
   float* lse;
   const int32_t* seqs;
-  int32_t batch, new_tokens, group, q_heads, rows, row_tiles, dim, window;
+  int32_t batch, new_tokens, group, q_heads, rows, row_tiles, dim, window, lead;
   float scale_log2;
   FastDiv group_div, head_div;  // head_div: by row_tiles
   int4* splits;                 // [blocks] the split segment whose first part a block holds (x < 0: none)
@@ -31,10 +31,9 @@ __device__ __forceinline__ float ex2(float x) {
 // e^(a - b) in base 2 where b is a maximum that may be -inf (nothing seen yet)
 __device__ __forceinline__ float ex2_diff(float a, float b) { return ex2(a - (b == -INFINITY ? 0.f : b)); }
 
-// The work is a list of units: for every (sequence, kv head, row tile) kLead units that stand for the cost of its
-// start and end (queries, join, write: about a chunk's time, measured 1 to 1.5 us against 1.5 us for 64 KB), then its
-// chunks of CH positions.  Blocks get equal runs of units; one that gets lead units alone has nothing to do there.
-constexpr int kLead = 1;
+// The work is a list of units: for every (sequence, kv head, row tile) `lead` units that stand for the cost of its start
+// and end (queries, join, write), then its chunks of CH positions.  Blocks get equal runs of units; one that gets lead
+// units alone has nothing to do there.
 
 // A run of chunks of one (sequence, kv head, row tile).
 struct Seg {
@@ -66,9 +65,9 @@ template <int CH>
 __device__ __forceinline__ bool open_seg(const AttnParams& p, Seg& s, int u0, int units, int align) {
   s.len = visible(p, s.b, &s.row, &s.lo);
   s.nch = chunks_of<CH>(s.len, s.lo, align);
-  s.c0 = max(0, u0 - kLead);
-  s.c1 = min(s.nch, u0 + units - kLead);
-  s.left = u0 + units - (s.nch + kLead);
+  s.c0 = max(0, u0 - p.lead);
+  s.c1 = min(s.nch, u0 + units - p.lead);
+  s.left = u0 + units - (s.nch + p.lead);
   s.t0 = (s.lo & -align) + s.c0 * CH;
   s.t1 = min(s.len, (s.lo & -align) + s.c1 * CH);
   return s.c1 > s.c0;
@@ -110,7 +109,7 @@ __device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_
   for (int b = b0; b < b1; ++b) {
     int row, lo;
     const int len = visible(p, b, &row, &lo);
-    units0 = kLead + chunks_of<CH>(len, lo, align);
+    units0 = p.lead + chunks_of<CH>(len, lo, align);
     mine += units0 * heads;
     if (cta == 0 && warp == (small ? 0 : warp) && (row < 0 || row >= p.kv.max_seqs)) atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
   }
@@ -149,7 +148,7 @@ __device__ __forceinline__ bool plan_run(const AttnParams& p, int align, int* s_
       for (;; ++b) {
         int row, lo;
         const int len = visible(p, b, &row, &lo);
-        units0 = kLead + chunks_of<CH>(len, lo, align);
+        units0 = p.lead + chunks_of<CH>(len, lo, align);
         if (b == b1 - 1 || run.u0 < at + units0 * heads) break;
         at += units0 * heads;
       }

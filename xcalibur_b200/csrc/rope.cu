@@ -12,6 +12,8 @@
 // a token are computed once per block and shared through shared memory.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "kv.cuh"
 
 namespace xcb {
@@ -33,224 +35,280 @@ struct RopeParams {
   const uint64_t* turns;
   KvLayer kv;                  // kv.k == null: no cache
   int32_t tokens, heads[3], dim, rot, interleaved, weight_f32;
-  int32_t block_tokens, block_heads;
+  int32_t block_tokens, groups[3];  // groups: rounds of heads of a kind, where a block takes one
   float eps, weight_offset, mscale;
 };
 
+// How a pair's two values lie: half the rotary dimension apart and that a multiple of 8 (partners are whole lanes), side
+// by side (in one lane), or any other way (through shared memory).
+enum Layout { kLanes, kPairs, kAny };
+
+// 1 / sqrt(x), x >= 0, within 2^-22.
+__device__ __forceinline__ float rsqrt_fast(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // LPH lanes hold one head (a power of two with 8 * LPH >= dim); F8: the cache holds e4m3.
-template <typename T, bool F8, int LPH>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
+//
+// Norm and rotation in one form: with r = rsqrt(mean(x^2) + eps), out[d] = r (x[d] A[d] + x[d'] B[d]), d' the other one
+// of d's pair, A[d] = w[d] cos, B[d] = +-w[d'] sin.  A lane makes its A and B once for all heads of its token, and
+// partners pass between lanes as they were read, two to a word.  Many tokens: blocks stay and walk over batches of
+// kMaxTok tokens, with the weights in shared memory as 32-bit values.
+template <typename T, bool F8, int LPH, Layout L>
+__global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int SLOTS = kThreads / LPH;
-  __shared__ float s_cos[kMaxTok][kMaxHalf];
-  __shared__ float s_sin[kMaxTok][kMaxHalf];
+  constexpr int NB = 4;                        // heads that a lane reads at once
+  __shared__ __align__(16) float s_cos[kMaxTok][kMaxHalf];
+  __shared__ __align__(16) float s_sin[kMaxTok][kMaxHalf];
+  __shared__ __align__(16) float s_w[2][kMaxHalf * 2];  // of queries and keys; 1 without a norm
   __shared__ int64_t s_row[kMaxTok];           // element offset of the token's row under kv head 0, or -1
-  __shared__ float s_x[SLOTS][LPH * 8];        // partners, where a pair is not 8 values apart
+  __shared__ float s_x[SLOTS][LPH * 8];        // partners, where a pair is not a multiple of 8 values apart
 
   const int tid = threadIdx.x;
   const int half = p.rot >> 1;
-  const int tok0 = blockIdx.x * p.block_tokens;
-  const int slot = tid / LPH, ln = tid % LPH, d0 = ln * 8;
+  const int slot = tid / LPH, d0 = (tid % LPH) * 8;
   const int per_tok = SLOTS / p.block_tokens;  // block_tokens is a power of two <= kMaxTok <= SLOTS
   const int bt = slot / per_tok;
-  const int tok = tok0 + bt;
-  const int nheads = p.heads[0] + p.heads[1] + p.heads[2];
-  const int h_begin = blockIdx.y * p.block_heads + slot % per_tok;
-  const int h_end = min(nheads, (int)(blockIdx.y + 1) * p.block_heads);
-  const bool live = tok < p.tokens && d0 < p.dim;
+  // Few tokens: a block has one round of heads of one kind; many: all heads of all kinds.
+  const int only = p.block_tokens == 1 ? (blockIdx.y < p.groups[0] ? 0 : blockIdx.y < p.groups[0] + p.groups[1] ? 1 : 2) : -1;
+  const int round = only < 0 ? 0 : blockIdx.y - (only > 0 ? p.groups[0] : 0) - (only > 1 ? p.groups[1] : 0);
 
-  const auto locate = [&](int h, int& kind, int& head) {
-    kind = h < p.heads[0] ? 0 : (h < p.heads[0] + p.heads[1] ? 1 : 2);
-    head = h - (kind > 0 ? p.heads[0] : 0) - (kind > 1 ? p.heads[1] : 0);
-  };
-  const auto load = [&](int h) -> uint4 {
-    if (!live || h >= h_end) return make_uint4(0, 0, 0, 0);
-    int kind, head;
-    locate(h, kind, head);
-    const T* x = (const T*)p.src[kind] + tok * p.tok_stride[kind] + head * p.head_stride[kind] + d0;
-    return *reinterpret_cast<const uint4*>(x);
-  };
-
-  uint4 next = load(h_begin);  // under way while the sines are computed
-
-  for (int i = tid; i < p.block_tokens * half; i += kThreads) {
-    const int b = i / half, j = i - b * half;
-    if (tok0 + b < p.tokens) {
-      const uint64_t phase = p.turns[j] * (uint64_t)(int64_t)p.positions[tok0 + b];
-      float sn, cs;
-      sincospif((float)(int32_t)(phase >> 32) * 4.656612873077393e-10f, &sn, &cs);  // 2^-31: turns * 2
-      s_cos[b][j] = cs * p.mscale;
-      s_sin[b][j] = sn * p.mscale;
+  if (only != 2) {
+    for (int i = tid; i < 2 * p.dim; i += kThreads) {
+      const int k = i >= p.dim, d = i - (k ? p.dim : 0);
+      const void* const w = p.weight[k];
+      s_w[k][d] = !w ? 1.f
+                  : p.weight_f32 ? ((const float*)w)[d] + p.weight_offset
+                                 : unpack2<T>(((const uint16_t*)w)[d]).x + p.weight_offset;
     }
   }
-  if (p.kv.k && tid < p.block_tokens) {
-    int64_t row = -1;
-    if (tok0 + tid < p.tokens) {
-      const int seq = p.seqs[tok0 + tid], pos = p.positions[tok0 + tid];
-      if (seq >= p.kv.max_seqs) {
-        atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
-      } else if (seq >= 0) {
-        const int pi = pos >= 0 ? fdiv(pos, p.kv.page_div) : p.kv.max_pages;
-        const int page = pi < p.kv.max_pages ? p.kv.table[(int64_t)seq * p.kv.max_pages + pi] : -1;
-        if (page < 0 || page >= p.kv.num_pages)
-          atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
-        else
-          row = ((int64_t)page * p.kv.kv_heads * p.kv.page_size + (pos - pi * p.kv.page_size)) * p.dim;
-      }
-    }
-    s_row[tid] = row;
-  }
-  __syncthreads();
+  const int lane = tid & 31;
+  int partner = lane;
+  if (L == kLanes && d0 < p.rot) partner = d0 < half ? lane + half / 8 : lane - half / 8;
+  const float inv_dim = 1.f / p.dim;
+  const auto other = [&](int d) { return d >= p.rot ? d : L == kPairs ? d ^ 1 : d < half ? d + half : d - half; };
 
-  // this lane's part of the rotation: out[j] = y[j] * c[j] + partner[j] * s[j]
-  float c[8], s[8], wq[8], wk[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int d = d0 + j;
-    c[j] = 1.f;
-    s[j] = 0.f;
-    if (d < p.rot) {
-      const int i = p.interleaved ? d >> 1 : (d < half ? d : d - half);
-      c[j] = s_cos[bt][i];
-      s[j] = s_sin[bt][i];
-      if (p.interleaved ? !(d & 1) : d < half) s[j] = -s[j];
-    }
-    wq[j] = wk[j] = 1.f;
-  }
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    if (p.weight[w] && d0 < p.dim) {
-      float* dst = w ? wk : wq;
-      if (p.weight_f32) {
-        const float* g = (const float*)p.weight[w] + d0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dst[j] = g[j] + p.weight_offset;
-      } else {
-        const uint4 g = *reinterpret_cast<const uint4*>((const T*)p.weight[w] + d0);
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2<T>(u[j]);
-          dst[2 * j] = f.x + p.weight_offset;
-          dst[2 * j + 1] = f.y + p.weight_offset;
+  int tok0 = blockIdx.x * p.block_tokens, tok = 0;
+  bool live = false;
+  // The batch's sines, and where its tokens go.
+  const auto prepare = [&]() {
+    if (only != 2) {  // values do not turn
+      for (int i = tid; i < p.block_tokens * half; i += kThreads) {
+        const int b = i / half, j = i - b * half;
+        if (tok0 + b < p.tokens) {
+          const uint64_t phase = p.turns[j] * (uint64_t)(int64_t)p.positions[tok0 + b];
+          float sn, cs;
+          sincospif((float)(int32_t)(phase >> 32) * 4.656612873077393e-10f, &sn, &cs);  // 2^-31: turns * 2
+          s_cos[b][j] = cs * p.mscale;
+          s_sin[b][j] = sn * p.mscale;
         }
       }
     }
-  }
-  const bool shuffled = !p.interleaved && (half & 7) == 0;
-  const int lane = tid & 31;
-  int partner = lane;
-  if (shuffled && d0 < p.rot) partner = d0 < half ? lane + half / 8 : lane - half / 8;
-  const float inv_dim = 1.f / p.dim;
+    if (p.kv.k && only != 0 && tid < p.block_tokens) {
+      int64_t row = -1;
+      if (tok0 + tid < p.tokens) {
+        const int seq = p.seqs[tok0 + tid], pos = p.positions[tok0 + tid];
+        if (seq >= p.kv.max_seqs) {
+          atomicOr(p.kv.status, XCB_STATUS_BAD_SEQ);
+        } else if (seq >= 0) {
+          const int pi = pos >= 0 ? fdiv(pos, p.kv.page_div) : p.kv.max_pages;
+          const int page = pi < p.kv.max_pages ? p.kv.table[(int64_t)seq * p.kv.max_pages + pi] : -1;
+          if (page < 0 || page >= p.kv.num_pages)
+            atomicOr(p.kv.status, XCB_STATUS_BAD_PAGE);
+          else
+            row = ((int64_t)page * p.kv.kv_heads * p.kv.page_size + (pos - pi * p.kv.page_size)) * p.dim;
+        }
+      }
+      s_row[tid] = row;
+    }
+  };
 
-  const int iters = (min(nheads, p.block_heads) + per_tok - 1) / per_tok;  // the same for every lane of a warp
-  int h = h_begin;
-  for (int it = 0; it < iters; ++it, h += per_tok) {
-    const uint4 raw = next;
-    next = load(h + per_tok);
-    const bool on = live && h < h_end;
-    int kind = 0, head = 0;
-    if (on) locate(h, kind, head);
-    float y[8];
-    {
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
+  const auto heads_of = [&](auto kind_tag) {
+    constexpr int KIND = decltype(kind_tag)::value;  // 0 queries, 1 keys, 2 values
+    const int heads = p.heads[KIND];
+    const int first = only < 0 ? slot % per_tok : round * SLOTS + slot;
+    const int rounds = only < 0 ? (heads + per_tok - 1) / per_tok : 1;  // the same for every lane of a warp
+    const T* const src = (const T*)p.src[KIND] + (live ? tok * p.tok_stride[KIND] + d0 : 0);
+    const T* at_src = src + first * p.head_stride[KIND];
+    const int64_t step = per_tok * p.head_stride[KIND];
+    uint4 raw[NB];
+    const auto load = [&](int i0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack2<T>(u[j]);
-        y[2 * j] = f.x;
-        y[2 * j + 1] = f.y;
+      for (int b = 0; b < NB; ++b) {
+        raw[b] = make_uint4(0, 0, 0, 0);
+        if (live && first + (i0 + b) * per_tok < heads && i0 + b < rounds) raw[b] = *reinterpret_cast<const uint4*>(at_src);
+        at_src += step;
+      }
+    };
+    load(0);
+    if (KIND == 0 || only > 0) {  // the reads are under way while the sines are computed
+      prepare();
+      __syncthreads();
+    }
+    float A[8], B[8];
+    if constexpr (KIND < 2) {
+      if (d0 < p.dim) {
+        const float* const w = s_w[KIND];
+        if (d0 >= p.rot) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) A[j] = w[d0 + j], B[j] = 0.f;
+        } else if constexpr (L == kLanes) {  // eight of one half: their sines, and their partners' weights, lie in a row
+          const int i = d0 < half ? d0 : d0 - half, o = d0 < half ? d0 + half : d0 - half;
+          const float sign = d0 < half ? -1.f : 1.f;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float4 c = *reinterpret_cast<const float4*>(&s_cos[bt][i + 4 * q]), sn = *reinterpret_cast<const float4*>(&s_sin[bt][i + 4 * q]);
+            const float4 a = *reinterpret_cast<const float4*>(w + d0 + 4 * q), e = *reinterpret_cast<const float4*>(w + o + 4 * q);
+            A[4 * q] = a.x * c.x, A[4 * q + 1] = a.y * c.y, A[4 * q + 2] = a.z * c.z, A[4 * q + 3] = a.w * c.w;
+            B[4 * q] = sign * e.x * sn.x, B[4 * q + 1] = sign * e.y * sn.y;
+            B[4 * q + 2] = sign * e.z * sn.z, B[4 * q + 3] = sign * e.w * sn.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int d = d0 + j;
+            A[j] = w[d];
+            B[j] = 0.f;
+            if (d < p.rot) {
+              const int i = L == kPairs ? d >> 1 : (d < half ? d : d - half);
+              A[j] *= s_cos[bt][i];
+              B[j] = w[other(d)] * s_sin[bt][i];
+              if (L == kPairs ? !(d & 1) : d < half) B[j] = -B[j];
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) A[j] = B[j] = 0.f;
       }
     }
-    if (p.weight[0] || p.weight[1]) {  // uniform: every lane takes part in the shuffles
-      float ss = 0.f;
+    T* at_q = (T*)p.q_out + (KIND == 0 ? tok * p.q_out_tok + first * p.q_out_head + d0 : 0);
+    const int64_t q_step = per_tok * p.q_out_head;
+    const int64_t row = KIND > 0 && p.kv.k && live ? s_row[bt] : -1;
+    uint8_t* const plane = p.kv.k + (KIND == 2 ? p.kv.plane : 0);
+    for (int i0 = 0; i0 < rounds; i0 += NB) {
+      if (i0) load(i0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+      for (int b = 0; b < NB; ++b) {
+        if (i0 + b >= rounds) break;
+        const int h = first + (i0 + b) * per_tok;
+        const bool on = live && h < heads;
+        const uint32_t w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+        uint4 w16 = raw[b];
+        float out[8];
+        if constexpr (KIND < 2) {
+          float x[8], y[8];
 #pragma unroll
-      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (kind < 2 && p.weight[kind]) {
-        const float r = rsqrtf(ss * inv_dim + p.eps);
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<T>(w[j]);
+            x[2 * j] = f.x;
+            x[2 * j + 1] = f.y;
+          }
+          if constexpr (L == kPairs) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (kind ? wk[j] : wq[j]);
+            for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+          } else if constexpr (L == kLanes) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack2<T>(__shfl_sync(0xffffffffu, w[j], partner));
+              y[2 * j] = f.x;
+              y[2 * j + 1] = f.y;
+            }
+          } else {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s_x[slot][d0 + j] = x[j];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = s_x[slot][other(d0 + j)];
+          }
+          float r = 1.f;
+          if (p.weight[KIND]) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+#pragma unroll
+            for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            r = rsqrt_fast(ss * inv_dim + p.eps);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) out[j] = r * (x[j] * A[j] + y[j] * B[j]);
+          w16 = make_uint4(pack2<T>(out[0], out[1]), pack2<T>(out[2], out[3]), pack2<T>(out[4], out[5]),
+                           pack2<T>(out[6], out[7]));
+        } else if constexpr (F8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<T>(w[j]);
+            out[2 * j] = f.x;
+            out[2 * j + 1] = f.y;
+          }
+        }
+        if constexpr (KIND == 0) {
+          if (on) *reinterpret_cast<uint4*>(at_q) = w16;
+          at_q += q_step;
+        } else {
+          if (!on) continue;
+          if (KIND == 1 && p.k_out) *reinterpret_cast<uint4*>((T*)p.k_out + tok * p.k_out_tok + h * p.k_out_head + d0) = w16;
+          if (row < 0) continue;
+          const int64_t at = row + (int64_t)h * p.kv.page_size * p.dim + d0;
+          if constexpr (F8) {
+            // Quantised from the 32-bit value, not from its 16-bit rounding.  Saturating conversion: infinities become
+            // +-448, NaN stays NaN.
+            const float* scales = KIND == 2 ? p.kv.v_scale : p.kv.k_scale;
+            const float sc = scales ? scales[h] : 1.f;
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              c[j] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(out[2 * j], sc), __fdiv_rn(out[2 * j + 1], sc)),
+                                              __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<uint2*>(plane + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+          } else {
+            *reinterpret_cast<uint4*>(plane + 2 * at) = w16;
+          }
+        }
       }
     }
-    float out[8];
-    if (p.interleaved) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = y[j] * c[j] + y[j ^ 1] * s[j];
-    } else if (shuffled) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = y[j] * c[j] + __shfl_sync(0xffffffffu, y[j], partner) * s[j];
-    } else {
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s_x[slot][d0 + j] = y[j];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int d = d0 + j;
-        const int q = d >= p.rot ? d : (d < half ? d + half : d - half);
-        out[j] = y[j] * c[j] + s_x[slot][q] * s[j];
-      }
-    }
-    if (!on) continue;
-    uint4 w16;
-    if (kind == 2) {
-      w16 = raw;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = y[j];
-    } else {
-      w16 = make_uint4(pack2<T>(out[0], out[1]), pack2<T>(out[2], out[3]), pack2<T>(out[4], out[5]),
-                       pack2<T>(out[6], out[7]));
-    }
-    if (kind == 0) {
-      if (p.q_out) *reinterpret_cast<uint4*>((T*)p.q_out + tok * p.q_out_tok + head * p.q_out_head + d0) = w16;
-      continue;
-    }
-    if (kind == 1 && p.k_out)
-      *reinterpret_cast<uint4*>((T*)p.k_out + tok * p.k_out_tok + head * p.k_out_head + d0) = w16;
-    if (!p.kv.k || s_row[bt] < 0) continue;
-    const int64_t at = s_row[bt] + (int64_t)head * p.kv.page_size * p.dim + d0;
-    uint8_t* plane = p.kv.k + (kind == 2 ? p.kv.plane : 0);
-    if constexpr (F8) {
-      // Quantised from the 32-bit value, not from its 16-bit rounding.  Saturating conversion: infinities become
-      // +-448, NaN stays NaN.
-      const float* scales = kind == 2 ? p.kv.v_scale : p.kv.k_scale;
-      const float sc = scales ? scales[head] : 1.f;
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(out[2 * j], sc), __fdiv_rn(out[2 * j + 1], sc)),
-                                        __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<uint2*>(plane + at) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-    } else {
-      *reinterpret_cast<uint4*>(plane + 2 * at) = w16;
-    }
+  };
+  for (;;) {
+    tok = tok0 + bt;
+    live = tok < p.tokens && d0 < p.dim;
+    if (only <= 0) heads_of(std::integral_constant<int, 0>{});
+    if (only < 0 || only == 1) heads_of(std::integral_constant<int, 1>{});
+    if (only < 0 || only == 2) heads_of(std::integral_constant<int, 2>{});
+    tok0 += gridDim.x * p.block_tokens;
+    if (tok0 >= p.tokens) break;
+    __syncthreads();  // the batch's sines have been read
   }
 }
 
-template <typename T, bool F8>
-int launch(RopeParams& p, cudaStream_t stream) {
+template <typename T, bool F8, Layout L>
+int launch_layout(RopeParams& p, cudaStream_t stream) {
   const int lph = p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 32;
   const int slots = kThreads / lph;
-  const int nheads = p.heads[0] + p.heads[1] + p.heads[2];
   const int sms = sm_count();
   if (!sms) return XCB_ERR_CUDA;
   // Few tokens: one head per lane group, so that a call is a single round of loads.  Many: four tokens per block,
   // each lane group walking over its token's heads with the cosines in registers.
-  const int groups = (nheads + slots - 1) / slots;
-  if ((int64_t)p.tokens * groups <= 8ll * sms) {
-    p.block_tokens = 1;
-    p.block_heads = slots;
-  } else {
-    p.block_tokens = kMaxTok;
-    p.block_heads = nheads;
-  }
-  const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens, (nheads + p.block_heads - 1) / p.block_heads);
+  int groups = 0;
+  for (int k = 0; k < 3; ++k) groups += p.groups[k] = (p.heads[k] + slots - 1) / slots;
+  const bool few = (int64_t)p.tokens * groups <= 8ll * sms && groups <= 65535;
+  p.block_tokens = few ? 1 : kMaxTok;
+  const int batches = (p.tokens + p.block_tokens - 1) / p.block_tokens;
+  const dim3 grid(few || batches < 3 * sms ? batches : 3 * sms, few ? groups : 1);
   switch (lph) {
-    case 8: rope_kernel<T, F8, 8><<<grid, kThreads, 0, stream>>>(p); break;
-    case 16: rope_kernel<T, F8, 16><<<grid, kThreads, 0, stream>>>(p); break;
-    default: rope_kernel<T, F8, 32><<<grid, kThreads, 0, stream>>>(p); break;
+    case 8: rope_kernel<T, F8, 8, L><<<grid, kThreads, 0, stream>>>(p); break;
+    case 16: rope_kernel<T, F8, 16, L><<<grid, kThreads, 0, stream>>>(p); break;
+    default: rope_kernel<T, F8, 32, L><<<grid, kThreads, 0, stream>>>(p); break;
   }
   return cudaGetLastError() == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
+}
+
+template <typename T, bool F8>
+int launch(RopeParams& p, cudaStream_t stream) {
+  if (p.interleaved) return launch_layout<T, F8, kPairs>(p, stream);
+  return p.rot % 16 ? launch_layout<T, F8, kAny>(p, stream) : launch_layout<T, F8, kLanes>(p, stream);
 }
 
 bool strides_ok(const void* p, const int64_t* s) { return kv_aligned(p, 16) && s[0] % 8 == 0 && s[1] % 8 == 0; }
@@ -269,6 +327,7 @@ extern "C" int xcb_qk_norm_rope(const XcbKvCache* c, const XcbRopeArgs* a, cudaS
       return XCB_ERR_INVALID_ARG;
     if (c->dtype != XCB_DTYPE_E4M3 && c->dtype != a->dtype) return XCB_ERR_UNSUPPORTED;
   }
+  if (a->tokens > 1 << 30) return XCB_ERR_UNSUPPORTED;
   if (a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0 || a->head_dim <= 0 || a->rotary_dim < 0 ||
       a->rotary_dim > a->head_dim || a->rotary_dim % 2 || !(a->eps >= 0.f))
     return XCB_ERR_INVALID_ARG;
