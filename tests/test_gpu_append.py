@@ -166,6 +166,21 @@ def test_e4m3_store_saturates_and_keeps_nan(cuda_device):
     assert got[:4].tolist() == [448.0, -448.0, 448.0, -448.0] and torch.isnan(got[4]) and got[5] == 0.3125
 
 
+@pytest.mark.parametrize("rot, interleaved", [(32, False), (12, False), (32, True), (12, True)])
+def test_what_does_not_turn_stays_as_it_is(cuda_device, rot, interleaved):
+    from xcalibur_b200 import Rope, qk_norm_rope
+
+    dev = cuda_device
+    q, _, _ = rows(dev, 9, 3, 1, 64, BF)
+    q[:, 1, 40] = float("inf")
+    q[:, 2, 63] = float("-inf")
+    q[:, 0, 33] = float("nan")
+    at = torch.arange(9, dtype=torch.int32, device=dev) + 5
+    got, _ = qk_norm_rope(q, None, at, Rope(rot, interleaved=interleaved, device=dev))
+    torch.testing.assert_close(got[..., rot:], q[..., rot:], rtol=0, atol=0, equal_nan=True)
+    assert torch.isfinite(got[..., :rot]).all()
+
+
 def test_tokens_without_a_page_are_not_stored(cuda_device):
     from xcalibur_b200 import PagedKVCache, Rope, _lib
 

@@ -19,9 +19,8 @@
 namespace xcb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTok = 4;     // tokens per block
-constexpr int kMaxHalf = 128;  // rotary_dim / 2
+constexpr int kThreads = 128;
+constexpr int kBlocks = 8;  // of an SM: 64 registers each thread
 
 struct RopeParams {
   const void* src[3];          // q, k, v
@@ -35,7 +34,7 @@ struct RopeParams {
   const uint64_t* turns;
   KvLayer kv;                  // kv.k == null: no cache
   int32_t tokens, heads[3], dim, rot, interleaved, weight_f32;
-  int32_t block_tokens, groups[3];  // groups: rounds of heads of a kind, where a block takes one
+  int32_t block_tokens, few, groups[3];  // groups: rounds of heads of a kind, where a block takes one
   float eps, weight_offset, mscale;
 };
 
@@ -54,25 +53,27 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
 //
 // Norm and rotation in one form: with r = rsqrt(mean(x^2) + eps), out[d] = r (x[d] A[d] + x[d'] B[d]), d' the other one
 // of d's pair, A[d] = w[d] cos, B[d] = +-w[d'] sin.  A lane makes its A and B once for all heads of its token, and
-// partners pass between lanes as they were read, two to a word.  Many tokens: blocks stay and walk over batches of
-// kMaxTok tokens, with the weights in shared memory as 32-bit values.
+// partners pass between lanes as they were read, two to a word.  Many tokens: blocks stay and walk over batches of up
+// to SLOTS tokens, with the weights in shared memory as 32-bit values.  The more tokens a batch has, the more heads use
+// a lane's A and B, and the fewer blocks have work: a batch has as many as leave two blocks an SM (1531 tokens of 10
+// heads of 128: 7.7 us with four, 9.8 with eight, 8.9 with two; 8192 of 40: 33.3 us with eight, 41.6 with four).
 template <typename T, bool F8, int LPH, Layout L>
-__global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocks) rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int SLOTS = kThreads / LPH;
   constexpr int NB = 4;                        // heads that a lane reads at once
-  __shared__ __align__(16) float s_cos[kMaxTok][kMaxHalf];
-  __shared__ __align__(16) float s_sin[kMaxTok][kMaxHalf];
-  __shared__ __align__(16) float s_w[2][kMaxHalf * 2];  // of queries and keys; 1 without a norm
-  __shared__ int64_t s_row[kMaxTok];           // element offset of the token's row under kv head 0, or -1
+  __shared__ __align__(16) float s_cos[SLOTS][LPH * 4];
+  __shared__ __align__(16) float s_sin[SLOTS][LPH * 4];
+  __shared__ __align__(16) float s_w[2][LPH * 8];  // of queries and keys; 1 without a norm
+  __shared__ int64_t s_row[SLOTS];             // element offset of the token's row under kv head 0, or -1
   __shared__ float s_x[SLOTS][LPH * 8];        // partners, where a pair is not a multiple of 8 values apart
 
   const int tid = threadIdx.x;
   const int half = p.rot >> 1;
   const int slot = tid / LPH, d0 = (tid % LPH) * 8;
-  const int per_tok = SLOTS / p.block_tokens;  // block_tokens is a power of two <= kMaxTok <= SLOTS
+  const int per_tok = SLOTS / p.block_tokens;  // block_tokens is a power of two <= SLOTS
   const int bt = slot / per_tok;
   // Few tokens: a block has one round of heads of one kind; many: all heads of all kinds.
-  const int only = p.block_tokens == 1 ? (blockIdx.y < p.groups[0] ? 0 : blockIdx.y < p.groups[0] + p.groups[1] ? 1 : 2) : -1;
+  const int only = p.few ? (blockIdx.y < p.groups[0] ? 0 : blockIdx.y < p.groups[0] + p.groups[1] ? 1 : 2) : -1;
   const int round = only < 0 ? 0 : blockIdx.y - (only > 0 ? p.groups[0] : 0) - (only > 1 ? p.groups[1] : 0);
 
   if (only != 2) {
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
   const int lane = tid & 31;
   int partner = lane;
   if (L == kLanes && d0 < p.rot) partner = d0 < half ? lane + half / 8 : lane - half / 8;
+  const uint32_t turned = d0 < p.rot ? ~0u : 0u;  // what does not turn adds 0, not 0 * infinity
   const float inv_dim = 1.f / p.dim;
   const auto other = [&](int d) { return d >= p.rot ? d : L == kPairs ? d ^ 1 : d < half ? d + half : d - half; };
 
@@ -208,11 +210,11 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
           }
           if constexpr (L == kPairs) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+            for (int j = 0; j < 8; ++j) y[j] = d0 + j < p.rot ? x[j ^ 1] : 0.f;
           } else if constexpr (L == kLanes) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 f = unpack2<T>(__shfl_sync(0xffffffffu, w[j], partner));
+              const float2 f = unpack2<T>(__shfl_sync(0xffffffffu, w[j], partner) & turned);
               y[2 * j] = f.x;
               y[2 * j + 1] = f.y;
             }
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
             for (int j = 0; j < 8; ++j) s_x[slot][d0 + j] = x[j];
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = s_x[slot][other(d0 + j)];
+            for (int j = 0; j < 8; ++j) y[j] = d0 + j < p.rot ? s_x[slot][other(d0 + j)] : 0.f;
           }
           float r = 1.f;
           if (p.weight[KIND]) {
@@ -289,14 +291,16 @@ int launch_layout(RopeParams& p, cudaStream_t stream) {
   const int slots = kThreads / lph;
   const int sms = sm_count();
   if (!sms) return XCB_ERR_CUDA;
-  // Few tokens: one head per lane group, so that a call is a single round of loads.  Many: four tokens per block,
-  // each lane group walking over its token's heads with the cosines in registers.
+  // Few tokens: one head per lane group, so that a call is a single round of loads.  Many: each lane group walks over
+  // heads of one token with its A and B in registers, in batches as large as leave two blocks an SM.
   int groups = 0;
   for (int k = 0; k < 3; ++k) groups += p.groups[k] = (p.heads[k] + slots - 1) / slots;
   const bool few = (int64_t)p.tokens * groups <= 8ll * sms && groups <= 65535;
-  p.block_tokens = few ? 1 : kMaxTok;
+  p.block_tokens = 1;
+  p.few = few;
+  while (!few && p.block_tokens < slots && p.tokens / (2 * p.block_tokens) >= 2 * sms) p.block_tokens *= 2;
   const int batches = (p.tokens + p.block_tokens - 1) / p.block_tokens;
-  const dim3 grid(few || batches < 3 * sms ? batches : 3 * sms, few ? groups : 1);
+  const dim3 grid(few || batches < kBlocks * sms ? batches : kBlocks * sms, few ? groups : 1);
   switch (lph) {
     case 8: rope_kernel<T, F8, 8, L><<<grid, kThreads, 0, stream>>>(p); break;
     case 16: rope_kernel<T, F8, 16, L><<<grid, kThreads, 0, stream>>>(p); break;

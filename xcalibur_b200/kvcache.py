@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -25,6 +26,13 @@ from ._lib import XcbAttnArgs, XcbKvCache, XcbRopeArgs, check
 _CACHE_DTYPES = {torch.bfloat16: _lib.XCB_DTYPE_BF16, torch.float16: _lib.XCB_DTYPE_F16,
                  torch.float8_e4m3fn: _lib.XCB_DTYPE_E4M3}
 _Q_DTYPES = {torch.bfloat16: _lib.XCB_DTYPE_BF16, torch.float16: _lib.XCB_DTYPE_F16}
+
+
+# The C structures of a call, packed in one go (a call's cost on the host is a good part of a short kernel's).
+_ROPE_ARGS = struct.Struct("8i3fi3P10q7P")
+_ATTN_ARGS = struct.Struct("6ifP3q3P")
+assert _ROPE_ARGS.size == ctypes.sizeof(XcbRopeArgs) and _ATTN_ARGS.size == ctypes.sizeof(XcbAttnArgs)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _check_ints(t: torch.Tensor, n: Optional[int], device: torch.device, what: str) -> torch.Tensor:
@@ -93,97 +101,130 @@ class Rope:
         return freqs, float(mscale)
 
 
-def _rows(t: torch.Tensor, heads: Optional[int], dim: Optional[int], tokens: Optional[int], what: str) -> torch.Tensor:
-    """[tokens, heads, dim] with contiguous, 16-byte aligned heads; copied where they are not."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim) or \
-            (tokens is not None and t.shape[0] != tokens):
-        raise ValueError(f"{what} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    a, b, c = t.stride()
-    if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+class _RopePlan:
+    """What one form of a call (types, shapes, strides, rotation) comes to: its checks passed, its constants packed."""
+
+    __slots__ = ("head", "strides", "q_shape", "k_shape")
 
 
-def _norm_weight(w: Optional[torch.Tensor], x: torch.Tensor, what: str):
-    if w is None:
-        return None
-    if w.shape != (x.shape[2],) or w.device != x.device or w.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"{what} must be [head_dim], of the queries' type or float32")
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-
-
-def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
+def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight_offset, q_out, k_out) -> _RopePlan:
     dtype = _Q_DTYPES.get(q.dtype)
     if dtype is None or not q.is_cuda:
         raise ValueError("queries must be bf16 or fp16 CUDA tensors (there is no CPU path)")
     device = q.device
-    q = _rows(q, None, None, None, "q")
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
     tokens, q_heads, dim = q.shape
+    if dim % 8:
+        check(_lib.XCB_ERR_UNSUPPORTED, "xcb_qk_norm_rope")
     kv_heads = cache.kv_heads if cache is not None else k.shape[1] if k is not None and k.dim() == 3 else 0
     for t, what in ((k, "k"), (v, "v")):
-        if t is not None and (t.dtype != q.dtype or t.device != device):
+        if t is None:
+            continue
+        if t.dtype != q.dtype or t.device != device:
             raise ValueError(f"{what} must have the queries' type and device")
-    k = None if k is None else _rows(k, kv_heads, dim, tokens, "k")
-    v = None if v is None else _rows(v, kv_heads, dim, tokens, "v")
+        if tuple(t.shape) != (tokens, kv_heads, dim):
+            raise ValueError(f"{what} must be [{tokens}, {kv_heads}, {dim}], got {tuple(t.shape)}")
     if rope.turns.device != device:
         raise ValueError("rope is on another device than the queries")
     if rope.rotary_dim > dim:
         raise ValueError(f"rotary_dim {rope.rotary_dim} is larger than head_dim {dim}")
-    positions = _check_ints(positions, tokens, device, "positions")
-    wq, wk = _norm_weight(q_weight, q, "q_weight"), _norm_weight(k_weight, q, "k_weight")
+    _check_ints(positions, tokens, device, "positions")
+    if cache is not None:
+        _check_ints(seqs, tokens, device, "seqs")
+    for w, what in ((wq, "q_weight"), (wk, "k_weight")):
+        if w is not None and (w.shape != (dim,) or w.device != device or w.dtype not in (q.dtype, torch.float32)):
+            raise ValueError(f"{what} must be [head_dim], of the queries' type or float32")
     if wq is not None and wk is not None and wq.dtype != wk.dtype:
         raise ValueError("q_weight and k_weight must have one type")
-    weight = wq if wq is not None else wk
-    outs = []
     for given, like, what in ((q_out, q, "q_out"), (k_out, k, "k_out")):
-        if given is None:
-            made = torch.empty(like.shape, dtype=q.dtype, device=device) if what == "q_out" or \
-                (cache is None and k is not None) else None
-        else:
-            if like is None or given.shape != like.shape or given.dtype != q.dtype or given.device != device or \
-                    _rows(given, None, None, None, what) is not given:
-                raise ValueError(f"{what} must be like its input, with aligned contiguous heads")
-            made = given
-        outs.append(made)
-    q_out, k_out = outs
-    a = XcbRopeArgs()
-    a.tokens, a.q_heads, a.kv_heads, a.head_dim = tokens, q_heads, kv_heads, dim
-    a.rotary_dim, a.interleaved, a.dtype = rope.rotary_dim, rope.interleaved, dtype
-    a.weight_dtype = dtype if weight is None or weight.dtype == q.dtype else _lib.XCB_DTYPE_F32
-    a.eps, a.weight_offset, a.mscale, a.layer = eps, weight_offset, rope.mscale, layer
-    a.q = q.data_ptr()
-    a.q_stride[:] = q.stride()[:2]
-    a.q_out = q_out.data_ptr()
-    a.q_out_stride[:] = q_out.stride()[:2]
-    if k is not None:
-        a.k = k.data_ptr()
-        a.k_stride[:] = k.stride()[:2]
-    if k_out is not None:
-        a.k_out = k_out.data_ptr()
-        a.k_out_stride[:] = k_out.stride()[:2]
-    if v is not None:
-        a.v = v.data_ptr()
-        a.v_stride[:] = v.stride()[:2]
-    if wq is not None:
-        a.q_weight = wq.data_ptr()
-    if wk is not None:
-        a.k_weight = wk.data_ptr()
-    a.positions, a.turns = positions.data_ptr(), rope.turns.data_ptr()
-    handle = None
-    if cache is not None:
-        seqs = _check_ints(seqs, tokens, device, "seqs")
-        a.seqs, handle = seqs.data_ptr(), cache._address
-    _launch(device, _lib.load().xcb_qk_norm_rope, "xcb_qk_norm_rope", handle, ctypes.addressof(a))
+        if given is not None and (like is None or given.shape != like.shape or given.dtype != q.dtype or
+                                  given.device != device or given.stride(2) != 1 or given.stride(0) % 8 or
+                                  given.stride(1) % 8):
+            raise ValueError(f"{what} must be like its input, with aligned contiguous heads")
+    weight = wq if wq is not None else wk
+    wtype = dtype if weight is None or weight.dtype == q.dtype else _lib.XCB_DTYPE_F32
+    plan = _RopePlan()
+    plan.head = (tokens, q_heads, kv_heads, dim, rope.rotary_dim, rope.interleaved, dtype, wtype, eps, weight_offset,
+                 rope.mscale, layer)
+
+    def strides(t):
+        return (0, 0) if t is None else t.stride()[:2]
+
+    made = (q_heads * dim, dim), (kv_heads * dim, dim)  # of outputs made here
+    plan.strides = strides(q) + strides(k) + strides(v) + (made[0] if q_out is None else strides(q_out)) + \
+        (made[1] if k_out is None else strides(k_out))
+    plan.q_shape = (tokens, q_heads, dim)
+    plan.k_shape = (tokens, kv_heads, dim) if cache is None and k is not None else None
+    return plan
+
+
+def _odd_rows(t: torch.Tensor) -> bool:
+    """Heads that the kernels cannot read in place: not contiguous, or not on 16-byte boundaries."""
+    a, b, c = t.stride() if t.dim() == 3 else (0, 0, 1)
+    return c != 1 or a % 8 != 0 or b % 8 != 0 or t.data_ptr() % 16 != 0
+
+
+# Calls' forms that have passed their checks: types, shapes and strides only, no tensor and no address.
+_PLANS: dict = {}
+
+
+def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
+    key = (None if cache is None else cache._key, layer, eps, weight_offset,
+           rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.device,
+           q.dtype, q.shape, q.stride(), q.device,
+           None if k is None else (k.dtype, k.shape, k.stride(), k.device),
+           None if v is None else (v.dtype, v.shape, v.stride(), v.device),
+           positions.dtype, positions.shape, positions.stride(), positions.device,
+           None if seqs is None else (seqs.dtype, seqs.shape, seqs.stride(), seqs.device),
+           None if q_weight is None else (q_weight.dtype, q_weight.shape, q_weight.stride(), q_weight.device),
+           None if k_weight is None else (k_weight.dtype, k_weight.shape, k_weight.stride(), k_weight.device),
+           None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride(), q_out.device),
+           None if k_out is None else (k_out.dtype, k_out.shape, k_out.stride(), k_out.device))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _rope_plan(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
+                          k_out)
+        copies = [t is not None and (_odd_rows(t) if i < 3 else not t.is_contiguous())
+                  for i, t in enumerate((q, k, v, positions, seqs, q_weight, k_weight))]
+        if any(copies):  # what cannot be read in place is copied, and the call is that of the copies
+            q, k, v, positions, seqs, q_weight, k_weight = (
+                t.clone(memory_format=torch.contiguous_format) if c else t
+                for t, c in zip((q, k, v, positions, seqs, q_weight, k_weight), copies))
+            return _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset,
+                              q_out, k_out)
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    if q_out is None:
+        q_out = torch.empty(plan.q_shape, dtype=q.dtype, device=q.device)
+    if k_out is None and plan.k_shape is not None:
+        k_out = torch.empty(plan.k_shape, dtype=q.dtype, device=q.device)
+    pq, pk, pv = q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr()
+    pwq, pwk = 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr()
+    if (pq | pk | pv | pwq | pwk) & 15:  # a view of the same form as one seen, but not on a 16-byte boundary
+        q, k, v, q_weight, k_weight = (t if t is None or t.data_ptr() % 16 == 0 else
+                                       t.clone(memory_format=torch.contiguous_format)
+                                       for t in (q, k, v, q_weight, k_weight))
+        return _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
+                          k_out)
+    if (q_out.data_ptr() | (0 if k_out is None else k_out.data_ptr())) & 15:
+        raise ValueError("q_out and k_out must be on 16-byte boundaries")
+    args = _ROPE_ARGS.pack(*plan.head, pq, pk, pv, *plan.strides, q_out.data_ptr(),
+                           0 if k_out is None else k_out.data_ptr(), pwq, pwk, positions.data_ptr(),
+                           0 if seqs is None else seqs.data_ptr(), rope.turns.data_ptr())
+    _launch(q.device, _lib.load().xcb_qk_norm_rope, "xcb_qk_norm_rope", None if cache is None else cache._address, args)
     return q_out, k_out
 
 
 def _launch(device, fn, what, *args):
     """Call a C entry on the device's current stream, with that device current."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, what)
 
@@ -243,8 +284,8 @@ class PagedKVCache:
             raise ValueError("the cache holds bf16, fp16 or e4m3")
         self.device = kv.device
         self.layers, _, self.num_pages, self.kv_heads, self.page_size, self.head_dim = kv.shape
-        for t, shape, what in ((table, (lens.numel(), table.shape[-1]), "page_table"), (lens, (table.shape[0],), "seq_lens"),
-                               (refs, (self.num_pages,), "refcounts")):
+        for t, shape, what in ((table, (lens.numel(), table.shape[-1]), "page_table"),
+                               (lens, (table.shape[0],), "seq_lens"), (refs, (self.num_pages,), "refcounts")):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device or not t.is_contiguous():
                 raise ValueError(f"{what} must be contiguous int32 {shape} on {self.device}")
         if not kv.is_contiguous():
@@ -269,6 +310,10 @@ class PagedKVCache:
                                   None if scales[0] is None else scales[0].data_ptr(),
                                   None if scales[1] is None else scales[1].data_ptr(), self.status.data_ptr())
         self._address = ctypes.addressof(self._struct)
+        # what a call's checks ask of the cache
+        self._key = (self.layers, self.kv_heads, self.head_dim, kv.dtype, self.device, self.max_seqs)
+        self._q_dtype = None if kv.dtype == torch.float8_e4m3fn else kv.dtype
+        self._plans: dict = {}
         self._attn_ws: dict = {}
         self._page_ws: dict = {}
         if self.lib.xcb_kv_workspace_bytes(self._address) == 0:
@@ -276,30 +321,31 @@ class PagedKVCache:
                              "values)")
 
     # -------------------------------------------------------------------------------------- workspaces
-    def _attn_workspace(self, q_heads: int, new_tokens: int) -> torch.Tensor:
-        """The current stream's workspace for this group and token count (counters and partial results)."""
-        key = (torch.cuda.current_stream(self.device).cuda_stream, q_heads, new_tokens)
+    def _attn_workspace(self, q_heads: int, new_tokens: int):
+        """The current stream's workspace for this group and token count (parts of split sequences): address, bytes."""
+        key = (_raw_stream(self.device.index), q_heads, new_tokens)
         ws = self._attn_ws.get(key)
         if ws is None:
             with torch.cuda.device(self.device):
                 nbytes = self.lib.xcb_attn_workspace_bytes(self._address, q_heads, new_tokens)
             if nbytes == 0:
-                raise ValueError(f"unsupported heads: {q_heads} query heads over {self.kv_heads}, {new_tokens} new tokens")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            _launch(self.device, self.lib.xcb_attn_workspace_init, "xcb_attn_workspace_init", ws.data_ptr(), nbytes)
-            self._attn_ws[key] = ws
-        return ws
+                raise ValueError(f"unsupported heads: {q_heads} query heads over {self.kv_heads}, {new_tokens} new "
+                                 "tokens")
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            _launch(self.device, self.lib.xcb_attn_workspace_init, "xcb_attn_workspace_init", buf.data_ptr(), nbytes)
+            ws = self._attn_ws[key] = (buf.data_ptr(), nbytes, buf)
+        return ws[:2]
 
-    def _page_workspace(self) -> torch.Tensor:
-        key = torch.cuda.current_stream(self.device).cuda_stream
+    def _page_workspace(self):
+        key = _raw_stream(self.device.index)
         ws = self._page_ws.get(key)
         if ws is None:
             nbytes = self.lib.xcb_kv_workspace_bytes(self._address)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            _launch(self.device, self.lib.xcb_kv_workspace_init, "xcb_kv_workspace_init", self._address, ws.data_ptr(),
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            _launch(self.device, self.lib.xcb_kv_workspace_init, "xcb_kv_workspace_init", self._address, buf.data_ptr(),
                     nbytes)
-            self._page_ws[key] = ws
-        return ws
+            ws = self._page_ws[key] = (buf.data_ptr(), nbytes, buf)
+        return ws[:2]
 
     # -------------------------------------------------------------------------------------- one layer's step
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -311,11 +357,11 @@ class PagedKVCache:
         must have been given to the sequences by ``extend``."""
         if k is None or v is None:
             raise ValueError("append needs keys and values")
-        if q.dim() == 3 and q.shape[2] != self.head_dim:
+        if q.shape[-1] != self.head_dim:
             raise ValueError(f"head_dim is {self.head_dim}")
         if q.device != self.device:
             raise ValueError("the queries are on another device than the cache")
-        if self.kv.dtype != torch.float8_e4m3fn and q.dtype != self.kv.dtype:
+        if q.dtype != self._q_dtype and self._q_dtype is not None:
             raise ValueError("the cache holds another type than the keys")
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
@@ -330,46 +376,66 @@ class PagedKVCache:
         [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
         ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
         natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
+        key = (layer, q.dtype, q.shape, q.stride(), q.device, window, scale,
+               None if seqs is None else (seqs.dtype, seqs.shape, seqs.stride(), seqs.device),
+               None if out is None else (out.dtype, out.shape, out.is_contiguous(), out.device))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._attend_plan(layer, q, seqs, window, scale, out)
+            if len(self._plans) >= 1024:
+                self._plans.clear()
+            self._plans[key] = plan
+        head, strides, shape, q_heads, new = plan
+        pq = q.data_ptr()
+        if strides is None or pq & 15:  # cannot be read in place: the call is that of a copy
+            return self.attend(layer, q.clone(memory_format=torch.contiguous_format), seqs=seqs, window=window,
+                               scale=scale, return_lse=return_lse, out=out)
+        if seqs is not None and not seqs.is_contiguous():
+            seqs = seqs.contiguous()
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        elif out.data_ptr() & 15:
+            raise ValueError("out must be on a 16-byte boundary")
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
+        if shape[0]:
+            ws, ws_bytes = self._attn_workspace(q_heads, new)
+            args = _ATTN_ARGS.pack(*head, pq, *strides, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                   0 if seqs is None else seqs.data_ptr())
+            _launch(self.device, self.lib.xcb_paged_attention, "xcb_paged_attention", self._address, args, ws, ws_bytes)
+        return (out, lse) if return_lse else out
+
+    def _attend_plan(self, layer, q, seqs, window, scale, out):
+        """A form of call checked: the constants of its argument block, the strides (None: q is to be copied), the
+        output's shape."""
         dtype = _Q_DTYPES.get(q.dtype)
         if dtype is None or q.device != self.device:
             raise ValueError(f"queries must be bf16 or fp16 on {self.device}")
-        single = q.dim() == 3
-        if single:
-            q = q.unsqueeze(1)
-        if q.dim() != 4 or q.shape[3] != self.head_dim:
+        shape = tuple(q.shape)
+        if len(shape) not in (3, 4) or shape[-1] != self.head_dim:
             raise ValueError(f"queries must be [batch, new_tokens, heads, {self.head_dim}]")
-        if self.kv.dtype != torch.float8_e4m3fn and q.dtype != self.kv.dtype:
+        s = q.stride()
+        if len(shape) == 3:
+            (batch, heads, dim), new, s = shape, 1, (s[0], 0, s[1], s[2])
+        else:
+            batch, new, heads, dim = shape
+        if self._q_dtype is not None and q.dtype != self._q_dtype:
             raise ValueError("the cache holds another type than the queries")
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
         if window < 0:
             raise ValueError("window must be >= 0")
-        batch, new, heads, dim = q.shape
         if heads == 0 or heads % self.kv_heads or new == 0:
             raise ValueError(f"query heads must be a multiple of {self.kv_heads}, new tokens at least 1")
-        s = q.stride()
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format)
-            s = q.stride()
         if seqs is not None:
-            seqs = _check_ints(seqs, batch, self.device, "seqs")
+            _check_ints(seqs, batch, self.device, "seqs")
         elif batch > self.max_seqs:
             raise ValueError(f"the cache has {self.max_seqs} sequences")
-        shape = (batch, heads, dim) if single else (batch, new, heads, dim)
-        if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
-        elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
-                or out.data_ptr() % 16:
+        if out is not None and (tuple(out.shape) != shape or out.dtype != q.dtype or out.device != self.device or
+                                not out.is_contiguous()):
             raise ValueError(f"out must be contiguous {shape}, of the queries' type")
-        lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
-        if batch:
-            a = XcbAttnArgs(batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else scale,
-                            q.data_ptr(), s[:3], out.data_ptr(), None if lse is None else lse.data_ptr(),
-                            None if seqs is None else seqs.data_ptr())
-            ws = self._attn_workspace(heads, new)
-            _launch(self.device, self.lib.xcb_paged_attention, "xcb_paged_attention", self._address,
-                    ctypes.addressof(a), ws.data_ptr(), ws.numel())
-        return (out, lse) if return_lse else out
+        head = (batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else float(scale))
+        strides = None if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 else tuple(s[:3])
+        return head, strides, shape, heads, new
 
     # -------------------------------------------------------------------------------------- pages
     def _list(self, t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
@@ -386,9 +452,8 @@ class PagedKVCache:
         in one call the first keeps it.  Too few free pages: nothing changes and XCB_STATUS_NO_PAGES is set."""
         seqs = self._list(seqs, None, "seqs")
         new_tokens = self._list(new_tokens, seqs.shape[0], "new_tokens")
-        ws = self._page_workspace()
         _launch(self.device, self.lib.xcb_kv_extend, "xcb_kv_extend", self._address, seqs.data_ptr(),
-                new_tokens.data_ptr(), seqs.shape[0], ws.data_ptr(), ws.numel())
+                new_tokens.data_ptr(), seqs.shape[0], *self._page_workspace())
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Sequence ``dst[i]``, empty before, becomes a copy of ``src[i]`` that shares its pages."""
@@ -412,8 +477,7 @@ class PagedKVCache:
 
     def compact(self) -> None:
         """Live pages move down into the free ids below them; the upper part of the pool is free afterwards."""
-        ws = self._page_workspace()
-        _launch(self.device, self.lib.xcb_kv_compact, "xcb_kv_compact", self._address, ws.data_ptr(), ws.numel())
+        _launch(self.device, self.lib.xcb_kv_compact, "xcb_kv_compact", self._address, *self._page_workspace())
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Contents of page ``src[i]`` to page ``dst[i]`` in all layers (no dst twice, none that is also a src)."""
