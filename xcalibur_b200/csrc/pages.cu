@@ -337,6 +337,7 @@ struct CopyParams {
 // A block copies a 16 KB piece of one page of one plane at a time.  Of a part-full page only the used tokens move: a
 // stretch of each head.
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int pairs = p.count ? *p.count : p.n;
   const int64_t items = (int64_t)pairs * p.planes * p.pieces;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
@@ -420,8 +421,17 @@ int launch_copy(const XcbKvCache* c, const int* src, const int* dst, const int* 
   if (!sms) return XCB_ERR_CUDA;
   const int64_t most = (int64_t)(n < c->num_pages ? n : c->num_pages) * p.planes * p.pieces;
   const int64_t grid = most < 8ll * sms ? most : 8ll * sms;
-  copy_kernel<<<(unsigned)grid, kCopyThreads, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
+  // Launched along with the kernel before it, whose end it waits for on the device.
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, copy_kernel, p) == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
 }
 
 int list_check(const XcbKvCache* c, const int32_t* a, const int32_t* b, int n) {

@@ -104,7 +104,7 @@ class Rope:
 class _RopePlan:
     """What one form of a call (types, shapes, strides, rotation) comes to: its checks passed, its constants packed."""
 
-    __slots__ = ("head", "strides", "q_shape", "k_shape")
+    __slots__ = ("head", "strides", "q_shape", "k_shape", "like")
 
 
 def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight_offset, q_out, k_out) -> _RopePlan:
@@ -114,6 +114,15 @@ def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight
     device = q.device
     if q.dim() != 3:
         raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    if cache is not None:
+        if q.shape[2] != cache.head_dim:
+            raise ValueError(f"head_dim is {cache.head_dim}")
+        if q.device != cache.device:
+            raise ValueError("the queries are on another device than the cache")
+        if q.dtype != cache._q_dtype and cache._q_dtype is not None:
+            raise ValueError("the cache holds another type than the keys")
+        if not 0 <= layer < cache.layers:
+            raise ValueError(f"layer must be in [0, {cache.layers})")
     tokens, q_heads, dim = q.shape
     if dim % 8:
         check(_lib.XCB_ERR_UNSUPPORTED, "xcb_qk_norm_rope")
@@ -155,6 +164,7 @@ def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight
     plan.strides = strides(q) + strides(k) + strides(v) + (made[0] if q_out is None else strides(q_out)) + \
         (made[1] if k_out is None else strides(k_out))
     plan.q_shape = (tokens, q_heads, dim)
+    plan.like = q.is_contiguous()  # so is an output like it
     plan.k_shape = (tokens, kv_heads, dim) if cache is None and k is not None else None
     return plan
 
@@ -170,18 +180,18 @@ _PLANS: dict = {}
 
 
 def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
-    key = (None if cache is None else cache._key, layer, eps, weight_offset,
-           rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.device,
-           q.dtype, q.shape, q.stride(), q.device,
-           None if k is None else (k.dtype, k.shape, k.stride(), k.device),
-           None if v is None else (v.dtype, v.shape, v.stride(), v.device),
-           positions.dtype, positions.shape, positions.stride(), positions.device,
-           None if seqs is None else (seqs.dtype, seqs.shape, seqs.stride(), seqs.device),
-           None if q_weight is None else (q_weight.dtype, q_weight.shape, q_weight.stride(), q_weight.device),
-           None if k_weight is None else (k_weight.dtype, k_weight.shape, k_weight.stride(), k_weight.device),
-           None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride(), q_out.device),
-           None if k_out is None else (k_out.dtype, k_out.shape, k_out.stride(), k_out.device))
-    plan = _PLANS.get(key)
+    plans = _PLANS if cache is None else cache._rope_plans
+    key = (layer, eps, weight_offset, rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.get_device(),
+           q.dtype, q.shape, q.stride(), q.get_device(),
+           k is not None and (k.dtype, k.shape, k.stride(), k.get_device()),
+           v is not None and (v.dtype, v.shape, v.stride(), v.get_device()),
+           positions.dtype, positions.shape, positions.stride(), positions.get_device(),
+           seqs is not None and (seqs.dtype, seqs.shape, seqs.stride(), seqs.get_device()),
+           q_weight is not None and (q_weight.dtype, q_weight.shape, q_weight.stride(), q_weight.get_device()),
+           k_weight is not None and (k_weight.dtype, k_weight.shape, k_weight.stride(), k_weight.get_device()),
+           q_out is not None and (q_out.dtype, q_out.shape, q_out.stride(), q_out.get_device()),
+           k_out is not None and (k_out.dtype, k_out.shape, k_out.stride(), k_out.get_device()))
+    plan = plans.get(key)
     if plan is None:
         plan = _rope_plan(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
                           k_out)
@@ -193,11 +203,11 @@ def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight,
                 for t, c in zip((q, k, v, positions, seqs, q_weight, k_weight), copies))
             return _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset,
                               q_out, k_out)
-        if len(_PLANS) >= 1024:
-            _PLANS.clear()
-        _PLANS[key] = plan
+        if len(plans) >= 1024:
+            plans.clear()
+        plans[key] = plan
     if q_out is None:
-        q_out = torch.empty(plan.q_shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q) if plan.like else torch.empty(plan.q_shape, dtype=q.dtype, device=q.device)
     if k_out is None and plan.k_shape is not None:
         k_out = torch.empty(plan.k_shape, dtype=q.dtype, device=q.device)
     pq, pk, pv = q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr()
@@ -213,14 +223,17 @@ def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight,
     args = _ROPE_ARGS.pack(*plan.head, pq, pk, pv, *plan.strides, q_out.data_ptr(),
                            0 if k_out is None else k_out.data_ptr(), pwq, pwk, positions.data_ptr(),
                            0 if seqs is None else seqs.data_ptr(), rope.turns.data_ptr())
-    _launch(q.device, _lib.load().xcb_qk_norm_rope, "xcb_qk_norm_rope", None if cache is None else cache._address, args)
+    if cache is None:
+        _launch(q.device, _lib.load().xcb_qk_norm_rope, "xcb_qk_norm_rope", None, args)
+    else:
+        _launch(cache.device, cache.lib.xcb_qk_norm_rope, "xcb_qk_norm_rope", cache._address, args)
     return q_out, k_out
 
 
 def _launch(device, fn, what, *args):
     """Call a C entry on the device's current stream, with that device current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
@@ -310,10 +323,9 @@ class PagedKVCache:
                                   None if scales[0] is None else scales[0].data_ptr(),
                                   None if scales[1] is None else scales[1].data_ptr(), self.status.data_ptr())
         self._address = ctypes.addressof(self._struct)
-        # what a call's checks ask of the cache
-        self._key = (self.layers, self.kv_heads, self.head_dim, kv.dtype, self.device, self.max_seqs)
         self._q_dtype = None if kv.dtype == torch.float8_e4m3fn else kv.dtype
-        self._plans: dict = {}
+        self._plans: dict = {}       # forms of call that have passed their checks, as _PLANS
+        self._rope_plans: dict = {}
         self._attn_ws: dict = {}
         self._page_ws: dict = {}
         if self.lib.xcb_kv_workspace_bytes(self._address) == 0:
@@ -357,14 +369,6 @@ class PagedKVCache:
         must have been given to the sequences by ``extend``."""
         if k is None or v is None:
             raise ValueError("append needs keys and values")
-        if q.shape[-1] != self.head_dim:
-            raise ValueError(f"head_dim is {self.head_dim}")
-        if q.device != self.device:
-            raise ValueError("the queries are on another device than the cache")
-        if q.dtype != self._q_dtype and self._q_dtype is not None:
-            raise ValueError("the cache holds another type than the keys")
-        if not 0 <= layer < self.layers:
-            raise ValueError(f"layer must be in [0, {self.layers})")
         return _rope_call(self, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
                           None)[0]
 
@@ -376,16 +380,16 @@ class PagedKVCache:
         [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
         ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
         natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
-        key = (layer, q.dtype, q.shape, q.stride(), q.device, window, scale,
-               None if seqs is None else (seqs.dtype, seqs.shape, seqs.stride(), seqs.device),
-               None if out is None else (out.dtype, out.shape, out.is_contiguous(), out.device))
+        key = (layer, q.dtype, q.shape, q.stride(), q.get_device(), window, scale,
+               seqs is not None and (seqs.dtype, seqs.shape, seqs.get_device()),
+               out is not None and (out.dtype, out.shape, out.is_contiguous(), out.get_device()))
         plan = self._plans.get(key)
         if plan is None:
             plan = self._attend_plan(layer, q, seqs, window, scale, out)
             if len(self._plans) >= 1024:
                 self._plans.clear()
             self._plans[key] = plan
-        head, strides, shape, q_heads, new = plan
+        head, strides, shape, q_heads, new, like = plan
         pq = q.data_ptr()
         if strides is None or pq & 15:  # cannot be read in place: the call is that of a copy
             return self.attend(layer, q.clone(memory_format=torch.contiguous_format), seqs=seqs, window=window,
@@ -393,7 +397,7 @@ class PagedKVCache:
         if seqs is not None and not seqs.is_contiguous():
             seqs = seqs.contiguous()
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q) if like else torch.empty(shape, dtype=q.dtype, device=self.device)
         elif out.data_ptr() & 15:
             raise ValueError("out must be on a 16-byte boundary")
         lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
@@ -435,7 +439,7 @@ class PagedKVCache:
             raise ValueError(f"out must be contiguous {shape}, of the queries' type")
         head = (batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else float(scale))
         strides = None if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 else tuple(s[:3])
-        return head, strides, shape, heads, new
+        return head, strides, shape, heads, new, q.is_contiguous()
 
     # -------------------------------------------------------------------------------------- pages
     def _list(self, t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
