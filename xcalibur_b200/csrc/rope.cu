@@ -7,9 +7,10 @@
 // product's low 64 bits are the exact fraction of a turn, and its leading 32 bits give the angle to 2^-32 turns at
 // any position.
 //
-// Bound: HBM (each value read once and written once).  A head is held by D / 8 lanes, 16 bytes each, so the norm is a
-// few shuffles; a lane keeps its 8 cosines, sines and weights in registers for all heads of its token.  The sines of
-// a token are computed once per block and shared through shared memory.
+// Bound: HBM for prompts (each value read once and written once; 8192 tokens of 40 heads of 128 move 170 MB in 33.6 us,
+// 76% of a copy's rate), latency for a decode step (one token 3.7 us, 64 tokens into 8 bits 4.9 us: a round of loads,
+// the page lookup and the stores).  A head is held by D / 8 lanes, 16 bytes each, so the norm is a few shuffles.  The
+// sines of a token are computed once per block and shared through shared memory.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -20,7 +21,6 @@ namespace xcb {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kBlocks = 8;  // of an SM: 64 registers each thread
 
 struct RopeParams {
   const void* src[3];          // q, k, v
@@ -42,6 +42,10 @@ struct RopeParams {
 // by side (in one lane), or any other way (through shared memory).
 enum Layout { kLanes, kPairs, kAny };
 
+// Blocks of an SM: 64 registers each thread, or 80 where 64 do not hold the quantiser or the other layouts.
+template <bool F8, Layout L>
+constexpr int kBlocks = F8 || L != kLanes ? 6 : 8;
+
 // 1 / sqrt(x), x >= 0, within 2^-22.
 __device__ __forceinline__ float rsqrt_fast(float x) {
   float y;
@@ -58,7 +62,7 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
 // a lane's A and B, and the fewer blocks have work: a batch has as many as leave two blocks an SM (1531 tokens of 10
 // heads of 128: 7.7 us with four, 9.8 with eight, 8.9 with two; 8192 of 40: 33.3 us with eight, 41.6 with four).
 template <typename T, bool F8, int LPH, Layout L>
-__global__ void __launch_bounds__(kThreads, kBlocks) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocks<F8, L>) rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int SLOTS = kThreads / LPH;
   constexpr int NB = 4;                        // heads that a lane reads at once
   __shared__ __align__(16) float s_cos[SLOTS][LPH * 4];
@@ -300,7 +304,7 @@ int launch_layout(RopeParams& p, cudaStream_t stream) {
   p.few = few;
   while (!few && p.block_tokens < slots && p.tokens / (2 * p.block_tokens) >= 2 * sms) p.block_tokens *= 2;
   const int batches = (p.tokens + p.block_tokens - 1) / p.block_tokens;
-  const dim3 grid(few || batches < kBlocks * sms ? batches : kBlocks * sms, few ? groups : 1);
+  const dim3 grid(few || batches < kBlocks<F8, L> * sms ? batches : kBlocks<F8, L> * sms, few ? groups : 1);
   switch (lph) {
     case 8: rope_kernel<T, F8, 8, L><<<grid, kThreads, 0, stream>>>(p); break;
     case 16: rope_kernel<T, F8, 16, L><<<grid, kThreads, 0, stream>>>(p); break;
