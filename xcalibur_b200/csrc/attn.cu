@@ -19,7 +19,12 @@
 // lane, swizzled so that ldmatrix has no bank conflicts, positions that are not there as zeros) and run ahead over the
 // ends of segments; up to eight consumer warps compute.  Consumers are WN groups of WM warps: a group takes its share
 // of a chunk's positions, the warps of a group 16 rows each (WM = 1, 2, 4, 8 for up to 128 rows).  Stages pass between
-// the two by mbarriers alone; groups meet at the end of a segment, where the rows' parts are joined.
+// the // the two by mbarriers alone; groups meet at the end of a segment, where the rows' parts are joined.
+//
+// Measured, 8 query heads a kv head of 128: one sequence of 131072 tokens 51 us (80% of a copy's rate), 64 of up to 8192
+// tokens 49 us (81%), 777 tokens 8.4 us (latency: plan, first stage, join kernel); 8 bits, 128 sequences 68.7 us (56%:
+// each value is converted to 16 bits before its tensor step); 4 draft tokens of 48 sequences, 20 rows 59 us (45%: 12 of
+// 32 rows of a tile are empty, and probabilities go in two parts).
 //
 // mma.sync m16n8k16 rather than tcgen05: with 16 rows a 16-bit chunk asks for an eighth of the former's rate, the rows
 // are the M of its step as they are, and its accumulators stay in the registers that the softmax needs them in.
@@ -71,20 +76,29 @@ __device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi)
       : "=r"(lo), "=r"(hi)
       : "r"(v));
 }
-template <int DP, bool F8>
+// An 8-bit cache of few rows: two blocks of half the warps, so that one computes while the other joins its warps' parts
+// at a segment's end (128 sequences: 85.3 -> 68.7 us).  A 16-bit one is bound by its copies, which then have half the
+// stages each: 48.8 -> 57.7 us (64 ragged sequences) with two.
+constexpr int blocks_per_sm(bool f8, int dp, int wm) { return f8 && dp < 256 && wm <= 2 ? 2 : 1; }
+
+template <int DP, bool F8, int WM>
 struct Shape {
-  static constexpr int kWarps = DP == 256 ? 4 : 8;   // consumers
+  static constexpr int kBlocks = blocks_per_sm(F8, DP, WM);  // of an SM
+  static constexpr int kWarps = DP == 256 || kBlocks == 2 ? 4 : 8;  // consumers
   static constexpr int kProducers = 4;               // registers are given out by four warps: fewer would not free any
   static constexpr int kThreads = (kWarps + kProducers) * 32;
+  // Two blocks of an SM start with 128 registers a thread; the consumers take over what the producers do not need.
+  static constexpr int kProducerRegs = 56, kConsumerRegs = 200;
+  static_assert(kBlocks == 1 || (kWarps == 4 && kProducerRegs + kConsumerRegs == 256), "what the block started with");
   static constexpr int kPitch = DP * (F8 ? 1 : 2);   // bytes of one position's row in shared memory
   static constexpr int kChunks = kPitch / 16;
   static constexpr int kTok = kPitch <= 128 ? 32 : 16;  // positions of a warp's step: 4 to 8 KB of keys and values
   static constexpr int kCh = kTok * kWarps;          // positions of a chunk
   static constexpr int kHalf = kCh * kPitch;         // a stage: its keys, then its values
-  static constexpr int kFit = 196608 / (2 * kHalf);
+  static constexpr int kFit = 196608 / kBlocks / (2 * kHalf);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kRing = kStages * 2 * kHalf;
-  static constexpr int kRedPitch = DP + 8;           // floats
+  static constexpr int kRedPitch = DP + (kBlocks == 2 ? 4 : 8);  // floats
   static constexpr int kSlots = kWarps / 2;
   static constexpr int kRed = kSlots * 16 * kRedPitch * 4;
   static constexpr int kRedMl = kSlots * 16 * 2 * 4;
@@ -105,9 +119,9 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {  // when this t
 }
 
 template <typename T, bool F8, int DP, int WM>
-__global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>::kBlocks) attn_kernel(const __grid_constant__ AttnParams p) {
   pdl_launch_dependents();
-  using S = Shape<DP, F8>;
+  using S = Shape<DP, F8, WM>;
   constexpr int NW = S::kWarps, WN = NW / WM, NS = S::kStages;
   constexpr int TOK = S::kTok, SN = TOK / 8;
   constexpr int CH = S::kCh;
@@ -155,6 +169,10 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
 
   if (warp >= NW) {
     // ---- producers: 32 positions at a time in turn -----------------------------------------------------------------------
+    if constexpr (S::kBlocks == 2) {
+      __syncwarp();
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kProducerRegs));
+    }
     constexpr int NP = S::kProducers, UN = (CH / 32 + NP - 1) / NP, RPI = 32 / S::kChunks;
     const int me = warp - NW;
     const int lc = lane % S::kChunks, lr = lane / S::kChunks;  // this lane copies 16 bytes at lc of rows lr, lr + RPI, ..
@@ -236,6 +254,10 @@ __global__ void __launch_bounds__(Shape<DP, F8>::kThreads, 1) attn_kernel(const 
   // ---- consumers -----------------------------------------------------------------------------------------------------
   const int grp = warp / WM, wm = warp % WM;
   const int g = lane >> 2, t = lane & 3;
+  if constexpr (S::kBlocks == 2) {
+    __syncwarp();
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kConsumerRegs));
+  }
   const int cta = blockIdx.x;
   // ldmatrix row addresses of this lane: keys as (position, dimension) pairs, values transposed
   const uint32_t k_lane = swz<S::kPitch>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
@@ -823,8 +845,10 @@ AttnWs attn_ws(int sms, int wm, int dp) {
 
 template <typename T, bool F8, int DP, int WM>
 int launch(const AttnParams& p, int sms, cudaStream_t stream) {
-  constexpr int bytes = Shape<DP, F8>::kBytes;
-  static_assert(bytes <= 227 * 1024, "the stages fit one SM");
+  using S = Shape<DP, F8, WM>;
+  constexpr int bytes = S::kBytes;
+  static_assert(S::kBlocks * (bytes + 1024) <= 228 * 1024, "the stages fit one SM");
+  sms *= S::kBlocks;  // from here on blocks
   static bool ready[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return XCB_ERR_CUDA;
@@ -832,9 +856,13 @@ int launch(const AttnParams& p, int sms, cudaStream_t stream) {
     if (cudaFuncSetAttribute(attn_kernel<T, F8, DP, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
         cudaSuccess)
       return XCB_ERR_CUDA;
+    // a block that started with fewer registers would wait for more without end
+    cudaFuncAttributes at{};
+    if (S::kBlocks == 2 && (cudaFuncGetAttributes(&at, attn_kernel<T, F8, DP, WM>) != cudaSuccess || at.numRegs != 128))
+      return XCB_ERR_CUDA;
     if (dev < kMaxDevices) ready[dev] = true;
   }
-  attn_kernel<T, F8, DP, WM><<<sms, Shape<DP, F8>::kThreads, bytes, stream>>>(p);
+  attn_kernel<T, F8, DP, WM><<<sms, S::kThreads, bytes, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return XCB_ERR_CUDA;
   // the join is launched along with it and waits on the device for its end
   cudaLaunchAttribute attr{};
@@ -869,6 +897,11 @@ int launch_dim(const AttnParams& p, int wm, int sms, cudaStream_t stream) {
   }
 }
 
+AttnWs ws_of(const XcbKvCache* c, int sms, int rows) {
+  const int wm = row_warps(rows, c->head_dim), dp = dim_class(c->head_dim);
+  return attn_ws(sms * blocks_per_sm(c->dtype == XCB_DTYPE_E4M3, dp, wm), wm, dp);
+}
+
 int heads_check(const XcbKvCache* c, int q_heads, int new_tokens) {
   if (q_heads <= 0 || new_tokens <= 0 || q_heads % c->kv_heads) return XCB_ERR_INVALID_ARG;
   if (q_heads > 65536 || new_tokens > 65536 || (int64_t)(q_heads / c->kv_heads) * new_tokens > 1 << 20)
@@ -886,7 +919,7 @@ extern "C" {
 size_t xcb_attn_workspace_bytes(const XcbKvCache* c, int32_t q_heads, int32_t new_tokens) {
   if (kv_check(c) != XCB_OK || heads_check(c, q_heads, new_tokens) != XCB_OK) return 0;
   const int sms = sm_count();
-  return sms ? attn_ws(sms, row_warps(q_heads / c->kv_heads * new_tokens, c->head_dim), dim_class(c->head_dim)).total : 0;
+  return sms ? ws_of(c, sms, q_heads / c->kv_heads * new_tokens).total : 0;
 }
 
 int xcb_attn_workspace_init(void* ws, size_t bytes, cudaStream_t stream) {
@@ -928,17 +961,17 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const int wm = row_warps(p.rows, p.dim);
   p.row_tiles = (p.rows + 16 * wm - 1) / (16 * wm);
-  // What a segment's ends cost in chunks.  64 ragged sequences, 8 rows: 52.4 / 48.9 / 49.9 us with 1 / 2 / 3; 8 bits, 128
-  // sequences, 8 rows: 102.7 / 85.4 / 87.4.  With more rows a chunk itself costs more: 4 draft tokens of 48 sequences, 20
-  // rows: 59.0 / 60.5 / 63.1.
-  p.lead = p.rows <= 16 ? 2 : 1;
+  // What a segment's ends cost in chunks.  64 ragged sequences, 8 rows: 52.1 / 48.8 / 49.6 / 50.3 us with 1 / 2 / 3 / 4.
+  // With more rows a chunk itself costs more: 4 draft tokens of 48 sequences, 20 rows: 58.9 with 1, 63.2 with 3.  Where an
+  // SM has two blocks, a chunk is half as long: 128 sequences in 8 bits, 8 rows: 90.7 / 75.2 / 68.7 / 69.8.
+  p.lead = (p.rows <= 16 ? 2 : 1) + blocks_per_sm(c->dtype == XCB_DTYPE_E4M3, dim_class(p.dim), wm) - 1;
   p.group_div = fast_div((uint32_t)p.group);
   p.head_div = fast_div((uint32_t)p.row_tiles);
   // a row of a layer's keys has a 32-bit index, the list of chunks a 31-bit one
   if ((int64_t)c->num_pages * c->kv_heads * c->page_size >= (1ll << 32) - 1 ||
       (int64_t)a->batch * c->kv_heads * p.row_tiles * ((int64_t)c->max_pages * c->page_size / 64 + 1 + p.lead) >= 1ll << 31)
     return XCB_ERR_UNSUPPORTED;
-  const AttnWs w = attn_ws(sms, wm, dim_class(p.dim));
+  const AttnWs w = ws_of(c, sms, p.rows);
   if (ws_bytes < w.total) return XCB_ERR_WORKSPACE;
   p.splits = (int4*)((uint8_t*)ws + w.splits);
   p.part_ml = (float*)((uint8_t*)ws + w.ml);
