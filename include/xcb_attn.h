@@ -49,7 +49,8 @@ typedef struct XcbKvCache {
  * fraction of 2^64: angles are exact modulo a full turn at any position.
  * With a cache, turned keys and the values go to slot positions[t] of sequence seqs[t] (seqs[t] < 0: padding, not
  * stored); e4m3 stores saturate at +-448 times the scale.  Two tokens of a call may not share a slot, and the
- * page must not be shared with another sequence (xcb_kv_extend sees to that).  q_out may be q, k_out may be k. */
+ * page must not be shared with another sequence (xcb_kv_extend sees to that).  q_out may be q, k_out may be k.
+ * At most 2^30 tokens a call. */
 typedef struct XcbRopeArgs {
   int32_t tokens, q_heads, kv_heads, head_dim;
   int32_t rotary_dim;               /* even, 0 <= rotary_dim <= head_dim                                   */
@@ -87,8 +88,10 @@ typedef struct XcbAttnArgs {
   float* lse;                       /* fp32 [batch, new_tokens, q_heads] or NULL                           */
   const int32_t* seqs;              /* [batch] or NULL                                                     */
 } XcbAttnArgs;
-/* Workspace of any call of this cache shape, group (q_heads / kv_heads) and new_tokens on the current device; zeroed
- * once with xcb_attn_workspace_init, kept consistent by the calls, which must be ordered on one stream. */
+/* Workspace of any call of this cache shape, group (q_heads / kv_heads) and new_tokens on the current device (parts of
+ * sequences that several blocks share), set up once with xcb_attn_workspace_init; calls that share one must be ordered
+ * on one stream.  XCB_ERR_UNSUPPORTED: 2^32 or more rows in one layer's keys (num_pages * kv_heads * page_size), or
+ * 2^31 or more chunks of 64 positions over all sequences, kv heads and row tiles. */
 size_t xcb_attn_workspace_bytes(const XcbKvCache* cache, int32_t q_heads, int32_t new_tokens);
 int xcb_attn_workspace_init(void* workspace, size_t bytes, cudaStream_t stream);
 int xcb_paged_attention(const XcbKvCache* cache, const XcbAttnArgs* args, void* workspace, size_t workspace_bytes,

