@@ -282,3 +282,13 @@ def test_refusals(cuda_device):
         PagedKVCache(1, 4, 2, 16, 64, max_seqs=2, max_pages=4, dtype=torch.float32, device=dev)
     with pytest.raises(ValueError):
         PagedKVCache(1, 4, 2, 16, 64, max_seqs=2, max_pages=4, device=dev, k_scale=torch.ones(2, device=dev))
+
+
+def test_a_scale_that_changes_in_place(cuda_device):
+    cache = make(cuda_device, [70], 1, 64, 16, BF)
+    q = queries(cuda_device, 1, 1, 2, 64, BF)
+    scale = torch.tensor(0.125)
+    first = cache.attend(0, q, scale=scale)
+    scale.mul_(4)
+    assert torch.equal(cache.attend(0, q, scale=scale), cache.attend(0, q, scale=0.5))
+    assert torch.equal(first, cache.attend(0, q, scale=0.125))

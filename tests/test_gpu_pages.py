@@ -183,3 +183,26 @@ def test_refusals(cuda_device):
         PagedKVCache.from_tensors(cache.kv[:, :1], cache.page_table, cache.seq_lens)
     with pytest.raises(ValueError):
         PagedKVCache.from_tensors(cache.kv, cache.page_table[:, :-1], cache.seq_lens)
+
+
+def test_first_extend_in_a_graph_and_calls_outside_it(cuda_device):
+    """A capture that makes the workspace does not leave one behind that only the graph has set up."""
+    from xcalibur_b200 import PagedKVCache
+
+    cache = PagedKVCache(1, 8, 1, 4, 16, max_seqs=2, max_pages=4, device=cuda_device)
+    seqs = torch.tensor([0, 1], dtype=torch.int32, device=cuda_device)
+    three = torch.full_like(seqs, 3)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        cache.extend(seqs, three)
+    with torch.cuda.stream(side):
+        cache.extend(seqs, three)
+        graph.replay()
+        cache.extend(seqs, three)
+        graph.replay()
+    side.synchronize()
+    assert cache.check_device_status() == 0
+    assert cache.seq_lens.tolist() == [12, 12]
+    assert sorted(cache.page_table[:, :3].flatten().tolist()) == [0, 1, 2, 3, 4, 5]

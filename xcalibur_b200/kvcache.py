@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+from operator import index
 from typing import Optional
 
 import torch
@@ -181,6 +182,7 @@ _PLANS: dict = {}
 
 def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
     plans = _PLANS if cache is None else cache._rope_plans
+    layer, eps, weight_offset = index(layer), float(eps), float(weight_offset)
     key = (layer, eps, weight_offset, rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.get_device(),
            q.dtype, q.shape, q.stride(), q.get_device(),
            k is not None and (k.dtype, k.shape, k.stride(), k.get_device()),
@@ -232,12 +234,12 @@ def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight,
 
 def _launch(device, fn, what, *args):
     """Call a C entry on the device's current stream, with that device current."""
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, _raw_stream(index))
+    on = device.index
+    if on == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(on))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, _raw_stream(on))
     if rc:
         check(rc, what)
 
@@ -328,6 +330,7 @@ class PagedKVCache:
         self._rope_plans: dict = {}
         self._attn_ws: dict = {}
         self._page_ws: dict = {}
+        self._captured: list = []
         if self.lib.xcb_kv_workspace_bytes(self._address) == 0:
             raise ValueError("unsupported cache shape (head_dim * element bytes must be a multiple of 16, at most 256 "
                              "values)")
@@ -356,7 +359,13 @@ class PagedKVCache:
             buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             _launch(self.device, self.lib.xcb_kv_workspace_init, "xcb_kv_workspace_init", self._address, buf.data_ptr(),
                     nbytes)
-            ws = self._page_ws[key] = (buf.data_ptr(), nbytes, buf)
+            ws = buf.data_ptr(), nbytes, buf
+            with torch.cuda.device(self.device):
+                capturing = torch.cuda.is_current_stream_capturing()
+            if capturing:  # zeroed when the graph runs, and so of no use to a call outside it
+                self._captured.append(buf)
+            else:
+                self._page_ws[key] = ws
         return ws[:2]
 
     # -------------------------------------------------------------------------------------- one layer's step
@@ -380,6 +389,9 @@ class PagedKVCache:
         [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
         ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
         natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
+        layer, window = index(layer), index(window)
+        if scale is not None:
+            scale = float(scale)
         key = (layer, q.dtype, q.shape, q.stride(), q.get_device(), window, scale,
                seqs is not None and (seqs.dtype, seqs.shape, seqs.get_device()),
                out is not None and (out.dtype, out.shape, out.is_contiguous(), out.get_device()))
