@@ -5,9 +5,9 @@
 // threads run (integer sums, minima, and prefix sums over lists).
 //
 // Bound: metadata calls are latency alone (one block, a few dependent rounds of memory: extend and truncate of 256
-// sequences 12.4 us with the copy's launch, which finds nothing to do); page copies are HBM, two bytes of traffic per
-// byte moved, in 16 KB pieces spread over the whole GPU (a pool of 1024 pages compacted in 138 us, 88% of a copy's
-// rate; the part-full pages of 192 forked sequences in 83 us, 75%, as stretches of each head).  The copy is launched
+// sequences 12.5 us with the copy's launch, which finds nothing to do); page copies are HBM, two bytes of traffic per
+// byte moved, in 16 KB pieces spread over the whole GPU (a pool of 1024 pages compacted in 126 us, 97% of a copy's
+// rate; the part-full pages of 192 forked sequences in 69 us, 91%, as stretches of each head).  The copy is launched
 // along with the planning kernel: 13.0 -> 12.4 us for the step.
 #include "kv.cuh"
 
@@ -423,7 +423,9 @@ int launch_copy(const XcbKvCache* c, const int* src, const int* dst, const int* 
   const int sms = sm_count();
   if (!sms) return XCB_ERR_CUDA;
   const int64_t most = (int64_t)(n < c->num_pages ? n : c->num_pages) * p.planes * p.pieces;
-  const int64_t grid = most < 8ll * sms ? most : 8ll * sms;
+  // Many short blocks rather than blocks that stay: the next one's list is read while others copy.  With 8 / 24 / 64 / 256
+  // an SM: fork's growth 82.2 / 69.6 / 68.6 / 77.8 us, compaction 137 / 131 / 126 / 128, a step without copies 12.1 / 12.5.
+  const int64_t grid = most < 64ll * sms ? most : 64ll * sms;
   // Launched along with the kernel before it, whose end it waits for on the device.
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
