@@ -41,7 +41,15 @@ namespace xcb {
 namespace {
 
 constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr float kSlack = 8.f;  // base 2, see attn_kernel's maximum
+// Exponentials are taken in base 2 against a reference kLift below a maximum that moves only when a score exceeds it by
+// more than kSlack (so the sums are rarely rescaled): up to 2^(kLift + kSlack).  As 32-bit sums and bf16 operands they
+// have the same relative accuracy at any size.  An f16 operand has a fixed step below 2^-14, so there the two fill its
+// upper range (2^15): a probability loses bits below 2^-25 of the largest one and is gone below 2^-36, e^-25.
+template <typename M>
+struct Reference {
+  static constexpr float kLift = std::is_same<M, __half>::value ? 11.f : 0.f;
+  static constexpr float kSlack = std::is_same<M, __half>::value ? 4.f : 8.f;
+};
 
 // the rest of the 16 bytes is zeroed; with bytes = 0 nothing is read
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -462,13 +470,13 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * to_log2[i];
         }
-        // A lazy maximum: exponentials are taken against a reference that moves only when a score exceeds it by kSlack,
-        // so the sums are rarely rescaled; up to 2^8 too large, they lose nothing in 32 bits, nor do the operands.
-        if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
+        // m is the reference that sums and exponentials are taken against, not the maximum itself.
+        constexpr float kLift = Reference<M>::kLift, kRise = kLift + Reference<M>::kSlack;
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + kRise || mx[1] > m[1] + kRise)) {
           float a[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float top = fmaxf(m[i], mx[i]);
+            const float top = fmaxf(m[i], mx[i] - kLift);
             a[i] = ex2_diff(m[i], top);
             m[i] = top;
             l[i] *= a[i];
@@ -547,8 +555,9 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
           continue;
         }
         // The probabilities as operands.  Rounded once to 16 bits they would add an error as large as the output's own
-        // rounding; for a 16-bit cache a second operand carries the rest.  An 8-bit cache's own rounding is coarser by
-        // far, and one f16 operand serves.
+        // rounding; for a 16-bit cache a second operand carries the rest: 2^-16 of a probability is left in bf16, 2^-22 in
+        // f16 (2^-36 of the largest one where that is more).  An 8-bit cache's own rounding is coarser by far, and one f16
+        // operand serves.
 #pragma unroll
         for (int b = 0; b < SN / 2; ++b) {
           uint32_t a_hi[4], a_lo[4];
