@@ -45,3 +45,33 @@ def test_small_probabilities_beside_a_large_one(cuda_device, dt, cdt, group, gap
     want = 64.0 * rest / (1 + rest)
     assert (out.double() - want).abs().max() <= want * (2.0 ** -10 + 2.0 ** -13 + ROUND[dt])
     assert (lse.double() - gap - math.log1p(rest)).abs().max() <= 2.0 ** -20 + n * 2.0 ** -23 + 2.0 ** -21 * gap
+
+
+@pytest.mark.parametrize("dt,cdt", [(BF, BF), (F16, F16), (BF, F8), (F16, F8)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_error_is_that_of_the_outputs_rounding(cuda_device, dt, cdt, new):
+    """The error against 64 bits, root of the mean square, beside that of the exact result rounded once.
+
+    Both are sums of many independent roundings.  Probabilities in two parts, scores and sums in 32 bits add less than
+    2^-15 to an output rounded to 2^-12.8 (f16) or more; in one f16 part (bf16 queries over e4m3) 2^-12.8 to 2^-9.8: less
+    than 3 % in quadrature either way.  One f16 part under an f16 output would add as much as its rounding (up to 41 %)."""
+    gen = torch.Generator().manual_seed(7)
+    kv = torch.randn((2, 2, 700, 128), generator=gen)
+    scales = {}
+    if cdt == F8:
+        kv = kv * 16
+        scales = {n: torch.tensor([s, 2 * s], device=cuda_device) for n, s in (("k_scale", 0.05), ("v_scale", 0.07))}
+    kv = kv.to(cdt)
+    cache = one_text(cuda_device, kv, 40, **scales)
+    q = torch.randn((40, new, 16, 128), generator=gen).to(dt).to(cuda_device)
+    out = cache.attend(0, q).double()
+    k, v = kv.double().to(cuda_device)
+    if scales:
+        k, v = (x * s.double()[:, None, None] for x, s in zip((k, v), scales.values()))
+    score = torch.einsum("blhgd,hnd->blhgn", q.double().view(40, new, 2, 8, 128), k) * 128 ** -0.5
+    at = torch.arange(700, device=cuda_device)
+    hidden = at > 700 - new + torch.arange(new, device=cuda_device)[:, None]
+    p = score.masked_fill(hidden[None, :, None, None], -math.inf).softmax(-1)
+    want = torch.einsum("blhgn,hnd->blhgd", p, v).reshape(40, new, 16, 128)
+    once = (want.to(dt).double() - want).square().mean().sqrt()
+    assert (out - want).square().mean().sqrt() <= 1.03 * once

@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
   constexpr int KS = DP / 16;       // 16-wide steps of the head dimension
   constexpr int NT = DP / 8;        // 8-wide column tiles of the output
   using M = typename std::conditional<F8, __half, T>::type;  // operand type of the tensor steps
+  constexpr bool kTwo = !F8 || std::is_same<T, __half>::value;  // probabilities in two parts, see the second product
   static_assert(WM <= NW && CH % 32 == 0, "a group has at most the block's warps");
 
   extern __shared__ __align__(1024) uint8_t smem[];  // all of the block's shared memory: stages start at multiples of 1 KB
@@ -554,10 +555,12 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
           }
           continue;
         }
-        // The probabilities as operands.  Rounded once to 16 bits they would add an error as large as the output's own
-        // rounding; for a 16-bit cache a second operand carries the rest: 2^-16 of a probability is left in bf16, 2^-22 in
-        // f16 (2^-36 of the largest one where that is more).  An 8-bit cache's own rounding is coarser by far, and one f16
-        // operand serves.
+        // The probabilities as operands.  Rounded once to their type they would add an error as large as the output's own
+        // rounding; a second operand carries the rest: 2^-16 of a probability is left in bf16, 2^-22 in f16 (2^-36 of the
+        // largest one where that is more).  bf16 queries over an 8-bit cache alone take one part: its f16 has three bits
+        // more than their output, whose error against 64 bits it raises from 0.001657 to 0.001664, and two parts take
+        // 74.9 us instead of 68.3 (128 sequences).  With f16 queries it would be 0.00026 instead of 0.00021, at 67.1 us
+        // instead of 74.4.
 #pragma unroll
         for (int b = 0; b < SN / 2; ++b) {
           uint32_t a_hi[4], a_lo[4];
@@ -565,7 +568,7 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
           for (int i = 0; i < 4; ++i) {
             const float x = s[2 * b + (i >> 1)][2 * (i & 1)], y = s[2 * b + (i >> 1)][2 * (i & 1) + 1];
             a_hi[i] = pack2<M>(x, y);
-            if constexpr (!F8) {
+            if constexpr (kTwo) {
               const float2 f = unpack2<M>(a_hi[i]);
               a_lo[i] = pack2<M>(x - f.x, y - f.y);
             }
@@ -584,6 +587,10 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
                 e4m3_f16(__byte_perm(w[2 * e], w[2 * e + 1], 0x7531), c0, c1);
                 mma16<M>(o[4 * n2 + 2 * e], a_hi, b0, b1);
                 mma16<M>(o[4 * n2 + 2 * e + 1], a_hi, c0, c1);
+                if constexpr (kTwo) {
+                  mma16<M>(o[4 * n2 + 2 * e], a_lo, b0, b1);
+                  mma16<M>(o[4 * n2 + 2 * e + 1], a_lo, c0, c1);
+                }
               } else {
                 mma16<M>(o[2 * n2 + e], a_hi, w[2 * e], w[2 * e + 1]);
                 mma16<M>(o[2 * n2 + e], a_lo, w[2 * e], w[2 * e + 1]);
