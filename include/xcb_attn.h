@@ -89,9 +89,10 @@ typedef struct XcbAttnArgs {
   const int32_t* seqs;              /* [batch] or NULL                                                     */
 } XcbAttnArgs;
 /* Workspace of any call of this cache shape, group (q_heads / kv_heads) and new_tokens on the current device (parts of
- * sequences that several blocks share), set up once with xcb_attn_workspace_init; calls that share one must be ordered
- * on one stream.  XCB_ERR_UNSUPPORTED: 2^32 or more rows in one layer's keys (num_pages * kv_heads * page_size), or
- * 2^31 or more chunks of 64 positions over all sequences, kv heads and row tiles. */
+ * sequences that several blocks share).  It needs no set-up (xcb_attn_workspace_init does nothing but refuse NULL), and
+ * one that is larger than asked for serves as well; calls that share one must be ordered.  XCB_ERR_UNSUPPORTED: 2^32 or
+ * more rows in one layer's keys (num_pages * kv_heads * page_size), or 2^31 or more chunks of 64 positions over all
+ * sequences, kv heads and row tiles. */
 size_t xcb_attn_workspace_bytes(const XcbKvCache* cache, int32_t q_heads, int32_t new_tokens);
 int xcb_attn_workspace_init(void* workspace, size_t bytes, cudaStream_t stream);
 int xcb_paged_attention(const XcbKvCache* cache, const XcbAttnArgs* args, void* workspace, size_t workspace_bytes,

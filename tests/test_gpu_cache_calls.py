@@ -1,0 +1,40 @@
+"""What calls on a cache keep and share: workspaces, checked forms, state."""
+import pytest
+import torch
+
+from tests import _attn_ref as ref
+from tests.test_gpu_attend import make, queries
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def test_workspaces_do_not_grow_with_the_lengths_of_prompts(cuda_device):
+    """Each number of new tokens is another form of call, of which a server sees hundreds; their scratch is shared."""
+    dev = cuda_device
+    cache = make(dev, [400], 1, 128, 64, BF)
+    q = queries(dev, 1, 300, 8, 128, BF)
+    cache.attend(0, q)
+    torch.cuda.synchronize(dev)
+    before = torch.cuda.memory_allocated(dev)
+    for new in range(1, 300):
+        cache.attend(0, q[:, :new])
+    # one buffer for 1, 2, 4 and 8 warps of rows each, 148 blocks of two parts of 16 rows of 128 floats a warp at most
+    assert len(cache._attn_ws) <= 4
+    assert torch.cuda.memory_allocated(dev) - before <= (1 + 2 + 4) * 160 * 2 * 16 * 132 * 4
+
+
+def test_a_workspace_holds_anything_at_first(cuda_device):
+    dev = cuda_device
+    lens = [3000, 1, 0, 777]
+    cache = make(dev, lens, 2, 128, 64, BF)
+    for new in (1, 5, 40):
+        q = queries(dev, len(lens), new, 16, 128, BF)
+        cache.attend(0, q)
+        for ws in cache._attn_ws.values():
+            ws.fill_(0xff)
+        out, lse = cache.attend(0, q, return_lse=True)
+        want, wlse, tol, ltol = ref.attend(cache.kv, cache.page_table, cache.seq_lens, q)
+        ref.assert_within(out, want, tol)
+        ref.assert_within(lse, wlse, ltol)

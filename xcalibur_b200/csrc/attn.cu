@@ -940,10 +940,8 @@ size_t xcb_attn_workspace_bytes(const XcbKvCache* c, int32_t q_heads, int32_t ne
   return sms ? ws_of(c, sms, q_heads / c->kv_heads * new_tokens).total : 0;
 }
 
-int xcb_attn_workspace_init(void* ws, size_t bytes, cudaStream_t stream) {
-  if (!ws) return XCB_ERR_INVALID_ARG;
-  return cudaMemsetAsync(ws, 0, bytes, stream) == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
-}
+// A call writes every record and part of its workspace before the join reads it.
+int xcb_attn_workspace_init(void* ws, size_t, cudaStream_t) { return ws ? XCB_OK : XCB_ERR_INVALID_ARG; }
 
 int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, size_t ws_bytes, cudaStream_t stream) {
   int rc = kv_check(c);

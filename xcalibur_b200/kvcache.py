@@ -336,20 +336,14 @@ class PagedKVCache:
                              "values)")
 
     # -------------------------------------------------------------------------------------- workspaces
-    def _attn_workspace(self, q_heads: int, new_tokens: int):
-        """The current stream's workspace for this group and token count (parts of split sequences): address, bytes."""
-        key = (_raw_stream(self.device.index), q_heads, new_tokens)
+    def _attn_workspace(self, nbytes: int) -> int:
+        """Address of the current stream's workspace of this size (parts of split sequences).  Sizes are few: one for
+        each number of warps that the rows of a kv head can take."""
+        key = (_raw_stream(self.device.index), nbytes)
         ws = self._attn_ws.get(key)
         if ws is None:
-            with torch.cuda.device(self.device):
-                nbytes = self.lib.xcb_attn_workspace_bytes(self._address, q_heads, new_tokens)
-            if nbytes == 0:
-                raise ValueError(f"unsupported heads: {q_heads} query heads over {self.kv_heads}, {new_tokens} new "
-                                 "tokens")
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            _launch(self.device, self.lib.xcb_attn_workspace_init, "xcb_attn_workspace_init", buf.data_ptr(), nbytes)
-            ws = self._attn_ws[key] = (buf.data_ptr(), nbytes, buf)
-        return ws[:2]
+            ws = self._attn_ws[key] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return ws.data_ptr()
 
     def _page_workspace(self):
         key = _raw_stream(self.device.index)
@@ -401,7 +395,7 @@ class PagedKVCache:
             if len(self._plans) >= 1024:
                 self._plans.clear()
             self._plans[key] = plan
-        head, strides, shape, q_heads, new, like = plan
+        head, strides, shape, ws_bytes, like = plan
         pq = q.data_ptr()
         if strides is None or pq & 15:  # cannot be read in place: the call is that of a copy
             return self.attend(layer, q.clone(memory_format=torch.contiguous_format), seqs=seqs, window=window,
@@ -414,7 +408,7 @@ class PagedKVCache:
             raise ValueError("out must be on a 16-byte boundary")
         lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
         if shape[0]:
-            ws, ws_bytes = self._attn_workspace(q_heads, new)
+            ws = self._attn_workspace(ws_bytes)
             args = _ATTN_ARGS.pack(*head, pq, *strides, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                    0 if seqs is None else seqs.data_ptr())
             _launch(self.device, self.lib.xcb_paged_attention, "xcb_paged_attention", self._address, args, ws, ws_bytes)
@@ -422,7 +416,7 @@ class PagedKVCache:
 
     def _attend_plan(self, layer, q, seqs, window, scale, out):
         """A form of call checked: the constants of its argument block, the strides (None: q is to be copied), the
-        output's shape."""
+        output's shape, the workspace's size."""
         dtype = _Q_DTYPES.get(q.dtype)
         if dtype is None or q.device != self.device:
             raise ValueError(f"queries must be bf16 or fp16 on {self.device}")
@@ -451,7 +445,11 @@ class PagedKVCache:
             raise ValueError(f"out must be contiguous {shape}, of the queries' type")
         head = (batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else float(scale))
         strides = None if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 else tuple(s[:3])
-        return head, strides, shape, heads, new, q.is_contiguous()
+        with torch.cuda.device(self.device):
+            ws_bytes = self.lib.xcb_attn_workspace_bytes(self._address, heads, new)
+        if ws_bytes == 0:
+            raise ValueError(f"unsupported heads: {heads} query heads over {self.kv_heads}, {new} new tokens")
+        return head, strides, shape, ws_bytes, q.is_contiguous()
 
     # -------------------------------------------------------------------------------------- pages
     def _list(self, t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
