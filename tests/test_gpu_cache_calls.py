@@ -38,3 +38,30 @@ def test_a_workspace_holds_anything_at_first(cuda_device):
         want, wlse, tol, ltol = ref.attend(cache.kv, cache.page_table, cache.seq_lens, q)
         ref.assert_within(out, want, tol)
         ref.assert_within(lse, wlse, ltol)
+
+
+def test_captures_of_page_calls_keep_no_memory(cuda_device):
+    """A server captures its steps again and again; each capture of a page call kept scratch of the pool's size."""
+    from xcalibur_b200 import PagedKVCache
+
+    dev = cuda_device
+    cache = PagedKVCache(1, 200000, 1, 1, 8, max_seqs=2, max_pages=4, device=dev)
+    seqs = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    none = torch.zeros_like(seqs)
+    side = torch.cuda.Stream(dev)
+    torch.cuda.synchronize(dev)
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            cache.extend(seqs, none)
+            cache.compact()
+        graph.replay()
+        torch.cuda.synchronize(dev)
+
+    capture()
+    before = torch.cuda.memory_allocated(dev)
+    for _ in range(5):
+        capture()
+    assert torch.cuda.memory_allocated(dev) - before < 1 << 20  # the scratch is 5.6 MB
+    assert cache.check_device_status() == 0

@@ -329,13 +329,15 @@ class PagedKVCache:
         self._plans: dict = {}       # forms of call that have passed their checks, as _PLANS
         self._rope_plans: dict = {}
         self._attn_ws: dict = {}
-        self._page_ws: dict = {}
-        self._captured: list = []
-        if self.lib.xcb_kv_workspace_bytes(self._address) == 0:
+        nbytes = self.lib.xcb_kv_workspace_bytes(self._address)
+        if nbytes == 0:
             raise ValueError("unsupported cache shape (head_dim * element bytes must be a multiple of 16, at most 256 "
-                             "values)")
+                             "values; kv on a 16-byte boundary; tables and lengths within 31 bits)")
+        # The page calls' workspace: zero between calls, which are ordered as they change the same tables.  Made here and
+        # not by the first call, which may be captured in a graph.
+        self._page_buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        self._page_ws = self._page_buf.data_ptr(), nbytes
 
-    # -------------------------------------------------------------------------------------- workspaces
     def _attn_workspace(self, nbytes: int) -> int:
         """Address of the current stream's workspace of this size (parts of split sequences).  Sizes are few: one for
         each number of warps that the rows of a kv head can take."""
@@ -344,23 +346,6 @@ class PagedKVCache:
         if ws is None:
             ws = self._attn_ws[key] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         return ws.data_ptr()
-
-    def _page_workspace(self):
-        key = _raw_stream(self.device.index)
-        ws = self._page_ws.get(key)
-        if ws is None:
-            nbytes = self.lib.xcb_kv_workspace_bytes(self._address)
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            _launch(self.device, self.lib.xcb_kv_workspace_init, "xcb_kv_workspace_init", self._address, buf.data_ptr(),
-                    nbytes)
-            ws = buf.data_ptr(), nbytes, buf
-            with torch.cuda.device(self.device):
-                capturing = torch.cuda.is_current_stream_capturing()
-            if capturing:  # zeroed when the graph runs, and so of no use to a call outside it
-                self._captured.append(buf)
-            else:
-                self._page_ws[key] = ws
-        return ws[:2]
 
     # -------------------------------------------------------------------------------------- one layer's step
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -467,7 +452,7 @@ class PagedKVCache:
         seqs = self._list(seqs, None, "seqs")
         new_tokens = self._list(new_tokens, seqs.shape[0], "new_tokens")
         _launch(self.device, self.lib.xcb_kv_extend, "xcb_kv_extend", self._address, seqs.data_ptr(),
-                new_tokens.data_ptr(), seqs.shape[0], *self._page_workspace())
+                new_tokens.data_ptr(), seqs.shape[0], *self._page_ws)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Sequence ``dst[i]``, empty before, becomes a copy of ``src[i]`` that shares its pages."""
@@ -491,7 +476,7 @@ class PagedKVCache:
 
     def compact(self) -> None:
         """Live pages move down into the free ids below them; the upper part of the pool is free afterwards."""
-        _launch(self.device, self.lib.xcb_kv_compact, "xcb_kv_compact", self._address, *self._page_workspace())
+        _launch(self.device, self.lib.xcb_kv_compact, "xcb_kv_compact", self._address, *self._page_ws)
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Contents of page ``src[i]`` to page ``dst[i]`` in all layers (no dst twice, none that is also a src)."""
