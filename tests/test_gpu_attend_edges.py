@@ -75,3 +75,46 @@ def test_error_is_that_of_the_outputs_rounding(cuda_device, dt, cdt, new):
     want = torch.einsum("blhgn,hnd->blhgd", p, v).reshape(40, new, 16, 128)
     once = (want.to(dt).double() - want).square().mean().sqrt()
     assert (out - want).square().mean().sqrt() <= 1.03 * once
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("group,new,dim,n", [(8, 1, 128, 40), (8, 1, 128, 20000), (5, 4, 80, 700), (128, 1, 128, 700),
+                                             (64, 4, 64, 9000), (16, 2, 256, 300), (64, 1, 256, 300)])
+def test_infinite_values_that_are_seen(cuda_device, dt, group, new, dim, n):
+    """Weights are positive, so an infinite value makes its dimension infinite, values of both signs or a NaN make it
+    NaN, wherever they stand and however the sequence is split; the other dimensions do not change."""
+    gen = torch.Generator().manual_seed(n)
+    kv = torch.randn((2, 2, n, dim), generator=gen).to(dt)
+    q = torch.randn((3, new, 2 * group, dim), generator=gen).to(dt).to(cuda_device)
+    plain = one_text(cuda_device, kv, 3).attend(0, q)
+    where = [0, n // 3, n // 2 + 5, n - new]
+    for i, at in enumerate(where):
+        kv[1, 1, at, 8 * i % dim] = math.inf
+        kv[1, 1, at, 8 * i % dim + 1] = -math.inf
+        kv[1, 1, at, 8 * i % dim + 3] = math.nan
+        kv[1, 1, at, 8 * i % dim + 6] = math.inf
+    kv[1, 1, n // 4, 6] = -math.inf
+    out, lse = one_text(cuda_device, kv, 3).attend(0, q, return_lse=True)
+    want = plain.clone()
+    for i in range(len(where)):
+        d = 8 * i % dim
+        want[:, :, group:, d] = math.inf
+        want[:, :, group:, d + 1] = -math.inf
+        want[:, :, group:, d + 3] = math.nan
+        want[:, :, group:, d + 6] = math.nan if d == 0 else math.inf
+    # other dimensions: rows of a tile that holds such values may be summed in another order
+    torch.testing.assert_close(out, want, rtol=2 * ROUND[dt], atol=2.0 ** -10, equal_nan=True)
+    assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+def test_infinite_values_outside_the_window(cuda_device, dt):
+    """The single token sees what its window holds; NaN and infinities in other heads, before it or past it stay out."""
+    n, window = 900, 64
+    kv = torch.randn((2, 1, n, 128), generator=torch.Generator().manual_seed(1)).to(dt)
+    kv[1, 0, n - window, 0] = math.inf
+    kv[1, 0, n - window - 1, :2] = -math.inf
+    kv[1, 0, :100] = math.nan
+    q = torch.randn((1, 8, 128), generator=torch.Generator().manual_seed(2)).to(dt).to(cuda_device)
+    out = one_text(cuda_device, kv, 1).attend(0, q, window=window)
+    assert (out[..., 0] == math.inf).all() and torch.isfinite(out[..., 1:]).all()

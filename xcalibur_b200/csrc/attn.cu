@@ -128,6 +128,13 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {  // when this t
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// A sum that came out as NaN although no score was one: an infinite value that a row sees makes its sum infinite, but the
+// tensor steps add it times the second part of a probability too, which may be zero or of either sign.  Such an output is
+// marked with a NaN of its own, and the join kernel looks through the values for what it should be.
+constexpr uint16_t kMark = 0x7ffe;
+template <typename T>
+constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+
 template <typename T, bool F8, int DP, int WM>
 __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>::kBlocks) attn_kernel(const __grid_constant__ AttnParams p) {
   pdl_launch_dependents();
@@ -161,6 +168,7 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
     }
     fence_mbar_init();
     *s_dead = 0;
+    p.marked[blockIdx.x] = make_int2(INT32_MAX, -1);
   }
   Run run;
   Seg cs;
@@ -622,6 +630,14 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
       const int tok = fdiv(r, p.group_div);
       return ((int64_t)cs.b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
     };
+    const auto mark = [&](T* at, float x, float y) {
+      uint16_t* const to = reinterpret_cast<uint16_t*>(at);
+      if (isnan(x)) to[0] = kMark;
+      if (isnan(y)) to[1] = kMark;
+      const int seg = cs.b * p.kv.kv_heads * p.row_tiles + cs.j;
+      atomicMin(&p.marked[cta].x, seg);
+      atomicMax(&p.marked[cta].y, seg);
+    };
     // A warp's part in a slot of the join buffer: rows of kRedPitch floats in the natural order of the dimensions, which
     // an 8-bit cache's accumulators hold four by four.
     const auto put = [&](int slot_) {
@@ -705,9 +721,14 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
         if (whole) {
           const int64_t at = place(tile0 + rl);
           const float inv = sum == 0.f ? 0.f : vs / sum;
-          if (d < p.dim)
-            *reinterpret_cast<uint2*>((T*)p.out + at * p.dim + d) =
-                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          if (d < p.dim) {
+            T* const dst = (T*)p.out + at * p.dim + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+            if (!F8 && isnan(acc.x + acc.y + acc.z + acc.w) && !isnan(sum)) {
+              mark(dst, acc.x, acc.y);
+              mark(dst + 2, acc.z, acc.w);
+            }
+          }
           if (p.lse && d == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
         } else {
           *reinterpret_cast<float4*>(p.part_o + ((int64_t)part_slot * RT + rl) * DP + d) = acc;
@@ -746,8 +767,10 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
               const float x = o[n + e][2 * i] * mul, y = o[n + e][2 * i + 1] * mul;
               if (!whole)
                 *reinterpret_cast<float2*>(po + d) = make_float2(x, y);
-              else if (d < p.dim)
+              else if (d < p.dim) {
                 *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(x, y);
+                if (isnan(x + y) && !isnan(l[i])) mark(dst + d, x, y);
+              }
             }
           }
         }
@@ -763,15 +786,60 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
   if (tid == 0) p.splits[cta] = split;
 }
 
+// Puts what they should be in the place of the marks in a segment's outputs (a warp a row, W dimensions a lane, as the
+// join): weights are positive, so infinite values of one sign are the result, values of both signs or a NaN among them
+// make it NaN.  One lane reads the columns of its dimensions: a path for values that are broken already.
+template <typename T, int W>
+__device__ __noinline__ void mend(const AttnParams& p, int rt, int b, int j) {
+  const int h = fdiv(j, p.head_div), tile0 = (j - h * p.row_tiles) * rt, d = (threadIdx.x & 31) * W;
+  int seq, first;
+  const int len = visible(p, b, &seq, &first);
+  if (d >= p.dim) return;
+  for (int r = tile0 + blockIdx.y * 8 + (threadIdx.x >> 5); r < min(tile0 + rt, p.rows); r += gridDim.y * 8) {
+    const int tok = fdiv(r, p.group_div);
+    const int64_t place = ((int64_t)b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
+    uint16_t* const out = (uint16_t*)p.out + place * p.dim + d;
+    uint32_t want = 0, up = 0, down = 0, nan = 0;  // a bit a dimension
+#pragma unroll
+    for (int w = 0; w < W; ++w) want |= (uint32_t)(out[w] == kMark) << w;
+    if (!want) continue;
+    const int end = len - p.new_tokens + tok + 1;
+    for (int pos = p.window && end > p.window ? end - p.window : 0; pos < end && ((nan | (up & down)) & want) != want; ++pos) {
+      const int pi = fdiv(pos, p.kv.page_div);
+      const int page = p.kv.table[(int64_t)seq * p.kv.max_pages + pi];
+      if (page < 0 || page >= p.kv.num_pages) continue;
+      const int64_t at = ((int64_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size);
+      const uint16_t* const v = reinterpret_cast<const uint16_t*>(p.kv.k + p.kv.plane) + at * p.dim + d;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t x = v[w];
+        if ((x & 0x7fffu) < kInf<T>) continue;
+        ((x & 0x7fffu) > kInf<T> ? nan : x >> 15 ? down : up) |= 1u << w;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (want >> w & 1) out[w] = (~nan & (up ^ down)) >> w & 1 ? (uint16_t)(kInf<T> | (down >> w & 1) << 15) : 0x7fff;
+  }
+}
+
 // Joins the parts of the split segment that block blockIdx.x of attn_kernel began, if it did: a warp takes a row at a
-// time, a lane DP / 32 dimensions, parts in run order.  Bound: latency, two or three rounds of reads.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams p, int rt) {
+// time, a lane DP / 32 dimensions, parts in run order.  And mends the outputs that the block marked.  Bound: latency, two
+// or three rounds of reads.  Two blocks an SM: with the registers that one takes when free, 444 blocks of a call run in
+// three rounds (verification 61.7 us instead of 59.1); three an SM spill (63.3).
+template <typename T, bool F8, int DP>
+__global__ void __launch_bounds__(256, 2) join_kernel(const __grid_constant__ AttnParams p, int rt) {
   constexpr int W = DP / 32, U = 64 / W;  // parts whose rows are read at once
   pdl_wait();
   const int4 sp = p.splits[blockIdx.x];
+  if constexpr (!F8) {
+    const int2 marked = p.marked[blockIdx.x];
+    const int heads = p.kv.kv_heads * p.row_tiles;
+    for (int seg = marked.x; seg <= marked.y; ++seg) mend<T, W>(p, rt, seg / heads, seg % heads);
+  }
   if (sp.x < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool odd = false;
   const int first = blockIdx.x, parts = sp.z - first + 1;
   const int h = fdiv(sp.y, p.head_div), tile0 = (sp.y - h * p.row_tiles) * rt;
   const int nrows = min(rt, p.rows - tile0);
@@ -834,8 +902,17 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
 #pragma unroll
     for (int w = 0; w < W; w += 2)
       if (lane * W + w < p.dim) *reinterpret_cast<uint32_t*>(dst + w) = pack2<T>(acc[w] * inv, acc[w + 1] * inv);
+    if constexpr (!F8) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (!isnan(acc[w]) || isnan(sum) || lane * W >= p.dim) continue;
+        reinterpret_cast<uint16_t*>(dst)[w] = kMark;
+        odd = true;
+      }
+    }
     if (p.lse && lane == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
   }
+  if (odd) mend<T, W>(p, rt, sp.x, sp.y);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -850,12 +927,13 @@ int row_warps(int rows, int dim) {
 }
 
 struct AttnWs {
-  size_t splits, ml, o, total;
+  size_t splits, marked, ml, o, total;
 };
 AttnWs attn_ws(int sms, int wm, int dp) {
   AttnWs w;
   w.splits = 0;
-  w.ml = ((size_t)sms * 16 + 255) / 256 * 256;
+  w.marked = (size_t)sms * 16;
+  w.ml = (w.marked + (size_t)sms * 8 + 255) / 256 * 256;
   w.o = w.ml + ((size_t)2 * sms * 16 * wm * 8 + 255) / 256 * 256;
   w.total = w.o + (size_t)2 * sms * 16 * wm * dp * 4;
   return w;
@@ -893,7 +971,7 @@ int launch(const AttnParams& p, int sms, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, DP>, p, rt) == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, join_kernel<T, F8, DP>, p, rt) == cudaSuccess ? XCB_OK : XCB_ERR_CUDA;
 }
 template <typename T, bool F8, int DP>
 int launch_wm(const AttnParams& p, int wm, int sms, cudaStream_t stream) {
@@ -990,6 +1068,7 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   const AttnWs w = ws_of(c, sms, p.rows);
   if (ws_bytes < w.total) return XCB_ERR_WORKSPACE;
   p.splits = (int4*)((uint8_t*)ws + w.splits);
+  p.marked = (int2*)((uint8_t*)ws + w.marked);
   p.part_ml = (float*)((uint8_t*)ws + w.ml);
   p.part_o = (float*)((uint8_t*)ws + w.o);
   if (c->dtype == XCB_DTYPE_E4M3)

@@ -19,6 +19,7 @@ struct AttnParams {
   float scale_log2;
   FastDiv group_div, head_div;  // head_div: by row_tiles
   int4* splits;                 // [blocks] the split segment whose first part a block holds (x < 0: none)
+  int2* marked;                 // [blocks] first and last segment that a block left marks in (x > y: none)
   float* part_ml;               // [2 * blocks][rows of a tile][2]
   float* part_o;                // [2 * blocks][rows of a tile][padded head_dim]
 };
