@@ -118,3 +118,15 @@ def test_infinite_values_outside_the_window(cuda_device, dt):
     q = torch.randn((1, 8, 128), generator=torch.Generator().manual_seed(2)).to(dt).to(cuda_device)
     out = one_text(cuda_device, kv, 1).attend(0, q, window=window)
     assert (out[..., 0] == math.inf).all() and torch.isfinite(out[..., 1:]).all()
+
+
+@pytest.mark.parametrize("dt,cdt", [(BF, BF), (F16, F8)])
+def test_a_scale_that_is_not_a_number_is_not_hidden(cuda_device, dt, cdt):
+    kv = torch.randn((2, 2, 70, 64), generator=torch.Generator().manual_seed(1)).to(cdt)
+    q = torch.randn((1, 2, 8, 64), generator=torch.Generator().manual_seed(2)).to(dt).to(cuda_device)
+    out, lse = one_text(cuda_device, kv, 1).attend(0, q, scale=math.nan, return_lse=True)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    if cdt == F8:
+        cache = one_text(cuda_device, kv, 1, k_scale=torch.tensor([1.0, math.nan], device=cuda_device))
+        out = cache.attend(0, q)
+        assert torch.isfinite(out[:, :, :4]).all() and torch.isnan(out[:, :, 4:]).all()

@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
         }
       }
     }
-    // Scores are multiplied by to_log2 after the maximum is taken, so it is made positive (and never zero: -inf stays).
+    // Scores are multiplied by to_log2 after the maximum is taken, so it is made positive (and never zero: -inf stays).  A
+    // NaN stays one.
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (to_log2[i] < 0.f) {
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
           qf[kk][2 + i] ^= 0x80008000u;
         }
       }
-      to_log2[i] = fmaxf(to_log2[i], 1e-37f);
+      if (to_log2[i] < 1e-37f) to_log2[i] = 1e-37f;
     }
   };
   // With an 8-bit cache the operands stay in shared memory, in the lanes' order, for all groups (in the join's buffer,
