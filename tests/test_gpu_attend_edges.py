@@ -130,3 +130,14 @@ def test_a_scale_that_is_not_a_number_is_not_hidden(cuda_device, dt, cdt):
         cache = one_text(cuda_device, kv, 1, k_scale=torch.tensor([1.0, math.nan], device=cuda_device))
         out = cache.attend(0, q)
         assert torch.isfinite(out[:, :, :4]).all() and torch.isnan(out[:, :, 4:]).all()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 40])
+def test_a_window_longer_than_any_sequence(cuda_device, window):
+    kv = torch.randn((2, 1, 3, 64), generator=torch.Generator().manual_seed(1)).to(BF)
+    cache = one_text(cuda_device, kv, 2)
+    q = torch.randn((2, 9, 4, 64), generator=torch.Generator().manual_seed(2)).to(BF).to(cuda_device)
+    out, lse = cache.attend(0, q, window=window, return_lse=True)  # the first six tokens see nothing
+    want, wlse = cache.attend(0, q, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    assert not out[:, :6].any() and (lse[:, :6] == -math.inf).all()

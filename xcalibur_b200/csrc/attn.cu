@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
       lo[i] = 0;
       if (p.new_tokens > 1 && r < p.rows) {
         hi[i] = cs.len - p.new_tokens + fdiv(r, p.group_div) + 1;
-        lo[i] = p.window ? max(0, hi[i] - p.window) : 0;
+        lo[i] = p.window && hi[i] > p.window ? hi[i] - p.window : 0;
       }
     }
     float to_log2[2];

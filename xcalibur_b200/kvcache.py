@@ -368,7 +368,7 @@ class PagedKVCache:
         [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
         ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
         natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
-        layer, window = index(layer), index(window)
+        layer, window = index(layer), min(index(window), 0x7fffffff)  # no sequence is longer
         if scale is not None:
             scale = float(scale)
         key = (layer, q.dtype, q.shape, q.stride(), q.get_device(), window, scale,
