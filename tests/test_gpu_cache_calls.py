@@ -65,3 +65,17 @@ def test_captures_of_page_calls_keep_no_memory(cuda_device):
         capture()
     assert torch.cuda.memory_allocated(dev) - before < 1 << 20  # the scratch is 5.6 MB
     assert cache.check_device_status() == 0
+
+
+def test_norm_of_a_head_whose_mean_square_is_below_the_normal_range(cuda_device):
+    """1e-38 is a 32-bit number, and without an epsilon its root divides."""
+    from xcalibur_b200 import Rope, qk_norm_rope
+
+    gen = torch.Generator().manual_seed(0)
+    q = (torch.randint(0, 2, (5, 3, 128), generator=gen) * 2 - 1).mul(1e-19).to(BF).to(cuda_device)
+    w = (1 + 0.1 * torch.randn(128, generator=gen)).to(BF).to(cuda_device)
+    at = torch.arange(5, dtype=torch.int32, device=cuda_device)
+    rope = Rope(64, device=cuda_device)
+    got, _ = qk_norm_rope(q, None, at, rope, q_weight=w, eps=0.0)
+    want, tol = ref.rope(q, at, rope.frequencies, 64, weight=w, eps=0.0)
+    ref.assert_within(got, want, ref.rounded_tol(want, tol, BF))

@@ -46,10 +46,10 @@ enum Layout { kLanes, kPairs, kAny };
 template <bool F8, Layout L>
 constexpr int kBlocks = F8 || L != kLanes ? 6 : 8;
 
-// 1 / sqrt(x), x >= 0, within 2^-22.
+// 1 / sqrt(x), x >= 0, within 2^-22, below the normal range too.
 __device__ __forceinline__ float rsqrt_fast(float x) {
   float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
