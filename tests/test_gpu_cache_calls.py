@@ -79,3 +79,33 @@ def test_norm_of_a_head_whose_mean_square_is_below_the_normal_range(cuda_device)
     got, _ = qk_norm_rope(q, None, at, rope, q_weight=w, eps=0.0)
     want, tol = ref.rope(q, at, rope.frequencies, 64, weight=w, eps=0.0)
     ref.assert_within(got, want, ref.rounded_tol(want, tol, BF))
+
+
+def test_a_form_of_call_is_checked_once_for_all_layers(cuda_device):
+    """The checked forms are kept up to a number; with one for each layer, a deep model's had room for few others."""
+    from xcalibur_b200 import Rope
+
+    dev = cuda_device
+    cache = make(dev, [20, 33], 2, 64, 16, BF, layers=5)
+    q = queries(dev, 2, 1, 4, 64, BF)
+    rope = Rope(64, device=dev)
+    at, seqs = cache.seq_lens - 1, torch.arange(2, dtype=torch.int32, device=dev)
+    new = torch.randn((2, 5, 2, 64), generator=torch.Generator().manual_seed(4)).to(BF).to(dev)
+    before = cache.kv.clone()
+    for layer in range(5):
+        q2 = cache.append(layer, q[:, 0], new[:, layer], new[:, layer], at, seqs, rope)
+        out = cache.attend(layer, q2)
+        want, _, tol, _ = ref.attend(cache.kv, cache.page_table, cache.seq_lens, q2[:, None], layer=layer)
+        ref.assert_within(out[:, None], want, tol)
+        for s in range(2):
+            p = int(cache.page_table[s, int(at[s]) // 16])
+            assert torch.equal(cache.kv[layer, 1, p, :, int(at[s]) % 16], new[s, layer])
+        # the layers that follow are untouched
+        raw = cache.kv[layer + 1:].view(torch.int16)
+        assert torch.equal(raw, before[layer + 1:].view(torch.int16))
+    assert len(cache._plans) == 1 and len(cache._rope_plans) == 1
+    for layer in (-1, 5):
+        with pytest.raises(ValueError):
+            cache.append(layer, q[:, 0], new[:, 0], new[:, 0], at, seqs, rope)
+        with pytest.raises(ValueError):
+            cache.attend(layer, q)

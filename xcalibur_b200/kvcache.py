@@ -108,7 +108,7 @@ class _RopePlan:
     __slots__ = ("head", "strides", "q_shape", "k_shape", "like")
 
 
-def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight_offset, q_out, k_out) -> _RopePlan:
+def _rope_plan(cache, q, k, v, positions, seqs, rope, wq, wk, eps, weight_offset, q_out, k_out) -> _RopePlan:
     dtype = _Q_DTYPES.get(q.dtype)
     if dtype is None or not q.is_cuda:
         raise ValueError("queries must be bf16 or fp16 CUDA tensors (there is no CPU path)")
@@ -122,8 +122,6 @@ def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight
             raise ValueError("the queries are on another device than the cache")
         if q.dtype != cache._q_dtype and cache._q_dtype is not None:
             raise ValueError("the cache holds another type than the keys")
-        if not 0 <= layer < cache.layers:
-            raise ValueError(f"layer must be in [0, {cache.layers})")
     tokens, q_heads, dim = q.shape
     if dim % 8:
         check(_lib.XCB_ERR_UNSUPPORTED, "xcb_qk_norm_rope")
@@ -156,7 +154,7 @@ def _rope_plan(cache, layer, q, k, v, positions, seqs, rope, wq, wk, eps, weight
     wtype = dtype if weight is None or weight.dtype == q.dtype else _lib.XCB_DTYPE_F32
     plan = _RopePlan()
     plan.head = (tokens, q_heads, kv_heads, dim, rope.rotary_dim, rope.interleaved, dtype, wtype, eps, weight_offset,
-                 rope.mscale, layer)
+                 rope.mscale)  # and the layer
 
     def strides(t):
         return (0, 0) if t is None else t.stride()[:2]
@@ -176,14 +174,16 @@ def _odd_rows(t: torch.Tensor) -> bool:
     return c != 1 or a % 8 != 0 or b % 8 != 0 or t.data_ptr() % 16 != 0
 
 
-# Calls' forms that have passed their checks: types, shapes and strides only, no tensor and no address.
+# Calls' forms that have passed their checks: types, shapes and strides only; no tensor, no address, no layer.
 _PLANS: dict = {}
 
 
 def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out, k_out):
     plans = _PLANS if cache is None else cache._rope_plans
     layer, eps, weight_offset = index(layer), float(eps), float(weight_offset)
-    key = (layer, eps, weight_offset, rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.get_device(),
+    if cache is not None and not 0 <= layer < cache.layers:
+        raise ValueError(f"layer must be in [0, {cache.layers})")
+    key = (eps, weight_offset, rope.rotary_dim, rope.interleaved, rope.mscale, rope.turns.get_device(),
            q.dtype, q.shape, q.stride(), q.get_device(),
            k is not None and (k.dtype, k.shape, k.stride(), k.get_device()),
            v is not None and (v.dtype, v.shape, v.stride(), v.get_device()),
@@ -195,7 +195,7 @@ def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight,
            k_out is not None and (k_out.dtype, k_out.shape, k_out.stride(), k_out.get_device()))
     plan = plans.get(key)
     if plan is None:
-        plan = _rope_plan(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
+        plan = _rope_plan(cache, q, k, v, positions, seqs, rope, q_weight, k_weight, eps, weight_offset, q_out,
                           k_out)
         copies = [t is not None and (_odd_rows(t) if i < 3 else not t.is_contiguous())
                   for i, t in enumerate((q, k, v, positions, seqs, q_weight, k_weight))]
@@ -222,7 +222,7 @@ def _rope_call(cache, layer, q, k, v, positions, seqs, rope, q_weight, k_weight,
                           k_out)
     if (q_out.data_ptr() | (0 if k_out is None else k_out.data_ptr())) & 15:
         raise ValueError("q_out and k_out must be on 16-byte boundaries")
-    args = _ROPE_ARGS.pack(*plan.head, pq, pk, pv, *plan.strides, q_out.data_ptr(),
+    args = _ROPE_ARGS.pack(*plan.head, layer, pq, pk, pv, *plan.strides, q_out.data_ptr(),
                            0 if k_out is None else k_out.data_ptr(), pwq, pwk, positions.data_ptr(),
                            0 if seqs is None else seqs.data_ptr(), rope.turns.data_ptr())
     if cache is None:
@@ -371,16 +371,18 @@ class PagedKVCache:
         layer, window = index(layer), min(index(window), 0x7fffffff)  # no sequence is longer
         if scale is not None:
             scale = float(scale)
-        key = (layer, q.dtype, q.shape, q.stride(), q.get_device(), window, scale,
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        key = (q.dtype, q.shape, q.stride(), q.get_device(), window, scale,
                seqs is not None and (seqs.dtype, seqs.shape, seqs.get_device()),
                out is not None and (out.dtype, out.shape, out.is_contiguous(), out.get_device()))
         plan = self._plans.get(key)
         if plan is None:
-            plan = self._attend_plan(layer, q, seqs, window, scale, out)
+            plan = self._attend_plan(q, seqs, window, scale, out)
             if len(self._plans) >= 1024:
                 self._plans.clear()
             self._plans[key] = plan
-        head, strides, shape, ws_bytes, like = plan
+        (head, rest), strides, shape, ws_bytes, like = plan
         pq = q.data_ptr()
         if strides is None or pq & 15:  # cannot be read in place: the call is that of a copy
             return self.attend(layer, q.clone(memory_format=torch.contiguous_format), seqs=seqs, window=window,
@@ -394,12 +396,12 @@ class PagedKVCache:
         lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
         if shape[0]:
             ws = self._attn_workspace(ws_bytes)
-            args = _ATTN_ARGS.pack(*head, pq, *strides, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            args = _ATTN_ARGS.pack(*head, layer, *rest, pq, *strides, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                    0 if seqs is None else seqs.data_ptr())
             _launch(self.device, self.lib.xcb_paged_attention, "xcb_paged_attention", self._address, args, ws, ws_bytes)
         return (out, lse) if return_lse else out
 
-    def _attend_plan(self, layer, q, seqs, window, scale, out):
+    def _attend_plan(self, q, seqs, window, scale, out):
         """A form of call checked: the constants of its argument block, the strides (None: q is to be copied), the
         output's shape, the workspace's size."""
         dtype = _Q_DTYPES.get(q.dtype)
@@ -415,8 +417,6 @@ class PagedKVCache:
             batch, new, heads, dim = shape
         if self._q_dtype is not None and q.dtype != self._q_dtype:
             raise ValueError("the cache holds another type than the queries")
-        if not 0 <= layer < self.layers:
-            raise ValueError(f"layer must be in [0, {self.layers})")
         if window < 0:
             raise ValueError("window must be >= 0")
         if heads == 0 or heads % self.kv_heads or new == 0:
@@ -428,7 +428,7 @@ class PagedKVCache:
         if out is not None and (tuple(out.shape) != shape or out.dtype != q.dtype or out.device != self.device or
                                 not out.is_contiguous()):
             raise ValueError(f"out must be contiguous {shape}, of the queries' type")
-        head = (batch, new, heads, dtype, layer, window, dim ** -0.5 if scale is None else float(scale))
+        head = (batch, new, heads, dtype), (window, dim ** -0.5 if scale is None else float(scale))  # the layer between
         strides = None if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 else tuple(s[:3])
         with torch.cuda.device(self.device):
             ws_bytes = self.lib.xcb_attn_workspace_bytes(self._address, heads, new)
