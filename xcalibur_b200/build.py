@@ -7,6 +7,7 @@ travels with the source tree.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -41,6 +42,20 @@ def needs_build() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+# Kernels of attn.cu whose warps hand registers to one another start with 128 a thread (launch bounds of two blocks of 256
+# threads); with fewer, the ones that take would wait for good, and the library refuses such calls.
+_SPLIT = re.compile(r"entry function '\S*attn_kernelI\S*Lb1ELi(?:64|128)ELi[12]E\S*' for.*?Used (\d+) registers", re.S)
+_SPLIT_KERNELS = 8
+
+
+def check_register_split(ptxas: str) -> None:
+    """Raise if the compiler's report (``-Xptxas -v``) gives one of these kernels other registers than it hands out."""
+    used = [int(n) for n in _SPLIT.findall(ptxas)]
+    if len(used) != _SPLIT_KERNELS or any((n + 7) // 8 * 8 != 128 for n in used):
+        raise RuntimeError(f"attn.cu: its {_SPLIT_KERNELS} kernels with a register split need 128 registers a thread, "
+                           f"the compiler gave {used}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
@@ -51,7 +66,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [nvcc(), *_flags(), "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+        split = src == "attn.cu"
+        done = subprocess.run(cmd + (["-Xptxas", "-v"] if split else []), stderr=subprocess.PIPE if split else None, text=True)
+        if split:
+            sys.stderr.writelines(line for line in done.stderr.splitlines(True) if not line.startswith(("ptxas info", "    ")))
+        done.check_returncode()
+        if split:
+            check_register_split(done.stderr)
         return obj
 
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
