@@ -154,3 +154,12 @@ def test_host_refusals():
                      Rope(64, device="cpu"))
     with pytest.raises(ValueError, match="no CPU path"):
         PagedKVCache(1, 1, 1, 16, 64, max_seqs=1, max_pages=1, device="cpu")
+
+
+def test_scaling_without_its_entries_is_refused():
+    """A factor alone was ignored: the rotation came out unscaled."""
+    for bad in ({"factor": 8.0}, {"type": None, "factor": 8.0}, {"type": "yarn", "factor": 4.0},
+                {"type": "linear", "factor": math.inf}, {"type": "linear", "factor": math.nan}):
+        with pytest.raises(ValueError):
+            Rope(64, scaling=bad, device="cpu")
+    assert Rope(64, scaling={}, device="cpu").frequencies == Rope(64, device="cpu").frequencies

@@ -72,9 +72,13 @@ class Rope:
 
     def _frequencies(self, scaling: dict):
         rot, base = self.rotary_dim, self.base
+        if scaling and scaling.get("type") is None:
+            raise ValueError("scaling needs a type")
         kind = scaling.pop("type", None)
+        if kind == "yarn" and "original" not in scaling:
+            raise ValueError("yarn needs the original context")
         factor = float(scaling.pop("factor", 1.0))
-        if not factor > 0:
+        if not (0 < factor < math.inf):
             raise ValueError("the scaling factor must be positive")
         mscale = 1.0
         if kind == "ntk":
