@@ -109,3 +109,22 @@ def test_a_form_of_call_is_checked_once_for_all_layers(cuda_device):
             cache.append(layer, q[:, 0], new[:, 0], new[:, 0], at, seqs, rope)
         with pytest.raises(ValueError):
             cache.attend(layer, q)
+
+
+def test_counts_of_a_callers_table(cuda_device):
+    """Entries past a sequence's last page, zeros in many a table, are not held pages."""
+    from xcalibur_b200 import PagedKVCache
+
+    dev = cuda_device
+    kv = torch.zeros((1, 2, 6, 1, 4, 8), dtype=BF, device=dev)
+    table = torch.tensor([[0, 1, 0, 0], [0, 0, 0, 0], [0, 2, 9, -1], [3, 0, 0, 0]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([5, 0, 10, 4], dtype=torch.int32, device=dev)
+    cache = PagedKVCache.from_tensors(kv, table, lens)
+    assert cache.refcounts.tolist() == [2, 1, 1, 1, 0, 0]
+    cache.free(torch.tensor([0, 3], dtype=torch.int32, device=dev))
+    assert cache.refcounts.tolist() == [1, 0, 1, 0, 0, 0]
+    for bad in (lens[:3], lens.long(), lens[:, None], lens.cpu()):
+        with pytest.raises(ValueError):
+            PagedKVCache.from_tensors(kv, table, bad)
+    with pytest.raises(ValueError):
+        PagedKVCache.from_tensors(kv, table[0], lens)

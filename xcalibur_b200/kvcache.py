@@ -284,16 +284,18 @@ class PagedKVCache:
     def from_tensors(cls, kv: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                      refcounts: Optional[torch.Tensor] = None, *, k_scale: Optional[torch.Tensor] = None,
                      v_scale: Optional[torch.Tensor] = None) -> "PagedKVCache":
-        """A cache over tensors that the caller holds.  Without ``refcounts`` they are counted from the table."""
+        """A cache over tensors that the caller holds.  Without ``refcounts`` they are counted from the table's entries
+        up to each sequence's length."""
         self = cls.__new__(cls)
         if kv.dim() != 6 or kv.shape[1] != 2:
             raise ValueError("kv must be [layers, 2, num_pages, kv_heads, page_size, head_dim]")
+        refs = torch.zeros(kv.shape[2], dtype=torch.int32, device=kv.device) if refcounts is None else refcounts
+        self._bind(kv, page_table, seq_lens, refs, k_scale, v_scale)
         if refcounts is None:
-            held = page_table.flatten()
-            held = held.masked_fill((held < 0) | (held >= kv.shape[2]), kv.shape[2]).long()
-            refcounts = torch.zeros(kv.shape[2] + 1, dtype=torch.int32, device=kv.device)
-            refcounts = refcounts.index_add_(0, held, torch.ones_like(held, dtype=torch.int32))[:-1]
-        self._bind(kv, page_table, seq_lens, refcounts, k_scale, v_scale)
+            page = page_table.clamp(0, self.num_pages - 1)
+            first = torch.arange(0, self.max_pages * self.page_size, self.page_size, device=self.device)
+            held = (page == page_table) & (first < seq_lens[:, None])
+            refs.index_add_(0, page.flatten(), held.flatten().int())
         return self
 
     def _bind(self, kv, table, lens, refs, k_scale, v_scale):
