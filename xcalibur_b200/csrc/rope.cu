@@ -46,10 +46,14 @@ enum Layout { kLanes, kPairs, kAny };
 template <bool F8, Layout L>
 constexpr int kBlocks = F8 || L != kLanes ? 6 : 8;
 
-// 1 / sqrt(x), x >= 0, within 2^-22, below the normal range too.
-__device__ __forceinline__ float rsqrt_fast(float x) {
+// 1 / sqrt(x), x >= 0, within 2^-22; x may be below the normal range if `tiny` (three more instructions: taken always, a
+// prompt of 8192 tokens is 33.7 us instead of 33.4).
+__device__ __forceinline__ float rsqrt_fast(float x, bool tiny) {
   float y;
-  asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  if (tiny)
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<F8, L>) rope_kernel(const __
             for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
 #pragma unroll
             for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrt_fast(ss * inv_dim + p.eps);
+            r = rsqrt_fast(ss * inv_dim + p.eps, p.eps < 1.2e-38f);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) out[j] = r * (x[j] * A[j] + y[j] * B[j]);
