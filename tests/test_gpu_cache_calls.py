@@ -128,3 +128,18 @@ def test_counts_of_a_callers_table(cuda_device):
             PagedKVCache.from_tensors(kv, table, bad)
     with pytest.raises(ValueError):
         PagedKVCache.from_tensors(kv, table[0], lens)
+
+
+def test_another_tensor_cannot_take_the_states_place(cuda_device):
+    """The kernels go by the tensors' addresses: one that was assigned would have been passed over in silence."""
+    cache = make(cuda_device, [20], 2, 64, 16, F8)
+    q = queries(cuda_device, 1, 1, 4, 64, BF)
+    for name in ("kv", "page_table", "seq_lens", "refcounts", "k_scale", "v_scale", "status"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
+    saved = cache.seq_lens.clone()
+    want = cache.attend(0, q)
+    cache.seq_lens.fill_(3)
+    assert not torch.equal(cache.attend(0, q), want)
+    cache.seq_lens.copy_(saved)
+    assert torch.equal(cache.attend(0, q), want)

@@ -266,7 +266,16 @@ class PagedKVCache:
     ``kv`` [layers, 2, num_pages, kv_heads, page_size, head_dim] in bf16, fp16 or e4m3; ``page_table`` int32 [max_seqs,
     max_pages] (-1: no page), ``seq_lens`` int32 [max_seqs], ``refcounts`` int32 [num_pages].  An e4m3 cache holds value
     / scale, ``k_scale`` and ``v_scale`` fp32 [kv_heads] (None: 1).  The tensors are the state: a caller may copy them,
-    set them back, or share them with its own code.  Calls on one cache must be ordered."""
+    set their contents back (``copy_``; another tensor cannot take their place), or share them with its own code.  Calls
+    on one cache, and replays of graphs that hold such calls, must be ordered."""
+
+    kv = property(lambda self: self._kv)
+    page_table = property(lambda self: self._page_table)
+    seq_lens = property(lambda self: self._seq_lens)
+    refcounts = property(lambda self: self._refcounts)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+    status = property(lambda self: self._status)
 
     def __init__(self, layers: int, num_pages: int, kv_heads: int, page_size: int, head_dim: int, *, max_seqs: int,
                  max_pages: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
@@ -320,16 +329,16 @@ class PagedKVCache:
                     raise ValueError(f"{what} must be float32 [{self.kv_heads}] on {self.device}")
                 t = t.contiguous()
             scales.append(t)
-        self.kv, self.page_table, self.seq_lens, self.refcounts = kv, table, lens, refs
-        self.k_scale, self.v_scale = scales
+        self._kv, self._page_table, self._seq_lens, self._refcounts = kv, table, lens, refs
+        self._k_scale, self._v_scale = scales
         self.max_seqs, self.max_pages = table.shape
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.lib = _lib.load()
         self._struct = XcbKvCache(self.layers, self.num_pages, self.kv_heads, self.page_size, self.head_dim,
                                   _CACHE_DTYPES[kv.dtype], self.max_seqs, self.max_pages, kv.data_ptr(),
                                   table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
                                   None if scales[0] is None else scales[0].data_ptr(),
-                                  None if scales[1] is None else scales[1].data_ptr(), self.status.data_ptr())
+                                  None if scales[1] is None else scales[1].data_ptr(), self._status.data_ptr())
         self._address = ctypes.addressof(self._struct)
         self._q_dtype = None if kv.dtype == torch.float8_e4m3fn else kv.dtype
         self._plans: dict = {}       # forms of call that have passed their checks, as _PLANS
