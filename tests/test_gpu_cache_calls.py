@@ -143,3 +143,20 @@ def test_another_tensor_cannot_take_the_states_place(cuda_device):
     assert not torch.equal(cache.attend(0, q), want)
     cache.seq_lens.copy_(saved)
     assert torch.equal(cache.attend(0, q), want)
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 2e-38])
+def test_norm_with_a_vanishing_epsilon(cuda_device, dt, eps):
+    from xcalibur_b200 import Rope, qk_norm_rope
+
+    gen = torch.Generator().manual_seed(3)
+    q = (torch.randn((4, 3, 96), generator=gen) * 2e-7).to(dt).to(cuda_device)
+    w = (1 + 0.1 * torch.randn(96, generator=gen)).to(dt).to(cuda_device)
+    at = torch.arange(4, dtype=torch.int32, device=cuda_device)
+    rope = Rope(96, device=cuda_device)
+    got, _ = qk_norm_rope(q, None, at, rope, q_weight=w, eps=eps)
+    want, tol = ref.rope(q, at, rope.frequencies, 96, weight=w, eps=eps)
+    ref.assert_within(got, want, ref.rounded_tol(want, tol, dt))
+    if eps:  # without one, zeros divide zero
+        assert not qk_norm_rope(torch.zeros_like(q), None, at, rope, q_weight=w, eps=eps)[0].any()

@@ -4,13 +4,14 @@
 // Mathematics: y = x * rsqrt(mean(x^2) + eps) * (w + offset); (a, b) -> (a cos - b sin, b cos + a sin) * mscale for
 // each pair of the first rotary_dim values.  The angle is position * f_i.  In 32 bits that product is off by up to
 // half a unit in its last place, 4e-3 radians at position 131072; here f_i / (2 pi) is a fraction of 2^64, so the
-// product's low 64 bits are the exact fraction of a turn, and its leading 32 bits give the angle to 2^-32 turns at
-// any position.
+// product's low 64 bits are the exact fraction of a turn; its leading 32 bits, rounded to a float's 24, give the angle
+// within 2^-26 turns (1e-7 radians) at any position.
 //
-// Bound: HBM for prompts (each value read once and written once; 8192 tokens of 40 heads of 128 move 170 MB in 33.6 us,
-// 76% of a copy's rate), latency for a decode step (one token 3.7 us, 64 tokens into 8 bits 4.9 us: a round of loads,
-// the page lookup and the stores).  A head is held by D / 8 lanes, 16 bytes each, so the norm is a few shuffles.  The
-// sines of a token are computed once per block and shared through shared memory.
+// Bound: HBM for prompts (each value read once and written once; 8192 tokens of 40 heads of 128 move 168 MB in 33.4 us,
+// 77% of a copy's rate; 48.7 us into 8 bits, 50%: two divisions a pair of values), latency for a decode step (one token
+// 3.7 us, 64 tokens into 8 bits 4.8 us: a round of loads, the page lookup and the stores).  A head is held by D / 8
+// lanes, 16 bytes each, so the norm is a few shuffles.  The sines of a token are computed once per block and shared
+// through shared memory.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -21,6 +22,7 @@ namespace xcb {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr float kSmall = 1.17549435e-38f;  // the smallest normal number
 
 struct RopeParams {
   const void* src[3];          // q, k, v
@@ -42,12 +44,13 @@ struct RopeParams {
 // by side (in one lane), or any other way (through shared memory).
 enum Layout { kLanes, kPairs, kAny };
 
-// Blocks of an SM: 64 registers each thread, or 80 where 64 do not hold the quantiser or the other layouts.
+// Blocks of an SM: 64 registers each thread, or 80 where 64 do not hold the quantiser or the other layouts (kAny spills 12
+// to 24 bytes of them even so).
 template <bool F8, Layout L>
 constexpr int kBlocks = F8 || L != kLanes ? 6 : 8;
 
-// 1 / sqrt(x), x >= 0, within 2^-22; x may be below the normal range if `tiny` (three more instructions: taken always, a
-// prompt of 8192 tokens is 33.7 us instead of 33.4).
+// 1 / sqrt(x), x >= 0, within 2^-22; x may be below the normal range if `tiny`: three more instructions, which taken always
+// would cost 1 % (a prompt of 8192 tokens 33.9 us instead of 33.5).
 __device__ __forceinline__ float rsqrt_fast(float x, bool tiny) {
   float y;
   if (tiny)
@@ -63,8 +66,8 @@ __device__ __forceinline__ float rsqrt_fast(float x, bool tiny) {
 // of d's pair, A[d] = w[d] cos, B[d] = +-w[d'] sin.  A lane makes its A and B once for all heads of its token, and
 // partners pass between lanes as they were read, two to a word.  Many tokens: blocks stay and walk over batches of up
 // to SLOTS tokens, with the weights in shared memory as 32-bit values.  The more tokens a batch has, the more heads use
-// a lane's A and B, and the fewer blocks have work: a batch has as many as leave two blocks an SM (1531 tokens of 10
-// heads of 128: 7.7 us with four, 9.8 with eight, 8.9 with two; 8192 of 40: 33.3 us with eight, 41.6 with four).
+// a lane's A and B, and the fewer blocks have work: a batch has as many as leave two blocks an SM (1531 tokens of 30
+// heads of 80: 7.4 us with four, 9.1 with eight, 8.3 with two; 8192 of 40 of 128: 33.5 us with eight, 36.4 with four).
 template <typename T, bool F8, int LPH, Layout L>
 __global__ void __launch_bounds__(kThreads, kBlocks<F8, L>) rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int SLOTS = kThreads / LPH;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<F8, L>) rope_kernel(const __
             for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
 #pragma unroll
             for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrt_fast(ss * inv_dim + p.eps, p.eps < 1.2e-38f);
+            r = rsqrt_fast(ss * inv_dim + p.eps, !std::is_same<T, __half>::value && p.eps < kSmall);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) out[j] = r * (x[j] * A[j] + y[j] * B[j]);
@@ -388,7 +391,9 @@ extern "C" int xcb_qk_norm_rope(const XcbKvCache* c, const XcbRopeArgs* a, cudaS
   p.rot = a->rotary_dim;
   p.interleaved = a->interleaved != 0;
   p.weight_f32 = a->weight_dtype == XCB_DTYPE_F32;
-  p.eps = a->eps;
+  // A mean square of f16 values is zero or at least 2^-56, so there an epsilon below the normal range may as well be at its
+  // edge: it keeps a head of zeros finite and changes nothing else.
+  p.eps = a->dtype == XCB_DTYPE_F16 && a->eps > 0.f && a->eps < kSmall ? kSmall : a->eps;
   p.weight_offset = a->weight_offset;
   p.mscale = a->mscale;
   const bool f8 = c && c->dtype == XCB_DTYPE_E4M3;
