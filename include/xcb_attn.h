@@ -78,7 +78,9 @@ int xcb_qk_norm_rope(const XcbKvCache* cache, const XcbRopeArgs* args, cudaStrea
  * already stored.  Token i stands at p = seq_lens - new_tokens + i and sees the positions j <= p, with a window only
  * p - window < j.  out = softmax(scale * q k^T) v per head; q head h reads kv head h / (q_heads / kv_heads).  A token
  * that sees nothing (an empty sequence, p < 0, no page) gets zeros and lse = -inf.  What is not seen is not read
- * into the result, whatever it holds.  lse (natural logarithm of the sum of exponentials) is optional. */
+ * into the result, whatever it holds; infinite values that are seen make their dimension infinite (NaN where both signs
+ * or a NaN are seen).  lse (natural logarithm of the sum of exponentials) is optional.  At most 65536 new tokens, 65536
+ * query heads, 2^20 sequences, and 2^20 rows (new_tokens * q_heads / kv_heads) a call. */
 typedef struct XcbAttnArgs {
   int32_t batch, new_tokens, q_heads, dtype, layer, window;  /* window 0: all                              */
   float scale;

@@ -8,9 +8,9 @@
 // Bound: HBM.  All rows of one kv head (group * new tokens) share one read of its keys and values, so a 16-bit cache
 // asks for `rows` flops per byte: 16 to 128, against ~255 where the tensor pipe would bound.
 //
-// Split: the work is cut into chunks of 16 * warps positions and the list of all chunks (sequence by sequence, head
-// by head) into as many equal runs as there are SMs, found on the device from the lengths, so that ragged batches and
-// single long sequences keep every SM busy alike and nothing waits for the host.  A (sequence, head) that lies in
+// Split: the work is cut into chunks of positions (16 or 32 for each consumer warp) and the list of all chunks (sequence
+// by sequence, head by head) into as many equal runs as there are blocks (one or two an SM), found on the device from the
+// lengths, so that ragged batches and single long sequences keep every SM busy alike and nothing waits for the host.  A (sequence, head) that lies in
 // several runs is joined by a second, small kernel, in run order, so results do not depend on timing; it is launched
 // along with the first and waits for it on the device.  (Joined by whichever block came last instead, 37 parts of
 // 131072 positions took one SM 7 us behind all others, and every part a fence and an atomic, 1 to 2 us.)
@@ -18,13 +18,16 @@
 // Inside a block four producer warps copy chunk after chunk into a ring of shared-memory stages (cp.async, 16 bytes a
 // lane, swizzled so that ldmatrix has no bank conflicts, positions that are not there as zeros) and run ahead over the
 // ends of segments; up to eight consumer warps compute.  Consumers are WN groups of WM warps: a group takes its share
-// of a chunk's positions, the warps of a group 16 rows each (WM = 1, 2, 4, 8 for up to 128 rows).  Stages pass between
-// the // the two by mbarriers alone; groups meet at the end of a segment, where the rows' parts are joined.
+// of a chunk's positions, the warps of a group 16 rows each (WM = 1, 2, 4, 8 for up to 128 rows; more rows are several
+// tiles, each over the whole range of positions that any row of the sequence sees).  Stages pass between the two by
+// mbarriers alone; groups meet at the end of a segment, where the rows' parts are joined.
 //
-// Measured, 8 query heads a kv head of 128: one sequence of 131072 tokens 51 us (80% of a copy's rate), 64 of up to 8192
-// tokens 49 us (81%), 777 tokens 8.4 us (latency: plan, first stage, join kernel); 8 bits, 128 sequences 68.7 us (56%:
-// each value is converted to 16 bits before its tensor step); 4 draft tokens of 48 sequences, 20 rows 59 us (45%: 12 of
-// 32 rows of a tile are empty, and probabilities go in two parts).
+// Measured, 8 query heads a kv head of 128: one sequence of 131072 tokens 51 us (80% of a copy's rate; 55 us on one GPU of
+// four), 64 of up to 8192 tokens 49 us (81%), 777 tokens 8.5 us (latency: plan, first stage, join kernel); 8 bits, 128
+// sequences 66 us (58%: each value is converted to 16 bits before its tensor step; f16 queries 73.5 us, whose probabilities
+// go in two parts); 4 draft tokens of 48 sequences, 20 rows 59 us (45%: 12 of 32 rows of a tile are empty, and
+// probabilities go in two parts).  A prompt of 4096 tokens, 4 kv heads, bf16: 3.1 ms, 3% of the dense products' rate for
+// what it has to compute, and no less under a window: tiles compute hidden positions too.
 //
 // mma.sync m16n8k16 rather than tcgen05: with 16 rows a 16-bit chunk asks for an eighth of the former's rate, the rows
 // are the M of its step as they are, and its accumulators stay in the registers that the softmax needs them in.  (A
@@ -87,7 +90,7 @@ __device__ __forceinline__ void e4m3_f16(uint32_t v, uint32_t& lo, uint32_t& hi)
       : "r"(v));
 }
 // An 8-bit cache of few rows: two blocks of half the warps, so that one computes while the other joins its warps' parts
-// at a segment's end (128 sequences: 85.3 -> 68.7 us).  A 16-bit one is bound by its copies, which then have half the
+// at a segment's end (128 sequences: 85.3 -> 66.3 us).  A 16-bit one is bound by its copies, which then have half the
 // stages each: 48.8 -> 57.7 us (64 ragged sequences) with two.
 constexpr int blocks_per_sm(bool f8, int dp, int wm) { return f8 && dp < 256 && wm <= 2 ? 2 : 1; }
 
@@ -568,8 +571,8 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
         // rounding; a second operand carries the rest: 2^-16 of a probability is left in bf16, 2^-22 in f16 (2^-36 of the
         // largest one where that is more).  bf16 queries over an 8-bit cache alone take one part: its f16 has three bits
         // more than their output, whose error against 64 bits it raises from 0.001657 to 0.001664, and two parts take
-        // 74.9 us instead of 68.3 (128 sequences).  With f16 queries it would be 0.00026 instead of 0.00021, at 67.1 us
-        // instead of 74.4.
+        // 73.1 us instead of 66.4 (128 sequences).  With f16 queries it would be 0.00026 instead of 0.00021, for the same
+        // tenth of the time.
 #pragma unroll
         for (int b = 0; b < SN / 2; ++b) {
           uint32_t a_hi[4], a_lo[4];
@@ -1060,9 +1063,10 @@ int xcb_paged_attention(const XcbKvCache* c, const XcbAttnArgs* a, void* ws, siz
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const int wm = row_warps(p.rows, p.dim);
   p.row_tiles = (p.rows + 16 * wm - 1) / (16 * wm);
-  // What a segment's ends cost in chunks.  64 ragged sequences, 8 rows: 52.1 / 48.8 / 49.6 / 50.3 us with 1 / 2 / 3 / 4.
-  // With more rows a chunk itself costs more: 4 draft tokens of 48 sequences, 20 rows: 58.9 with 1, 63.2 with 3.  Where an
-  // SM has two blocks, a chunk is half as long: 128 sequences in 8 bits, 8 rows: 90.7 / 75.2 / 68.7 / 69.8.
+  // What a segment's ends cost in chunks.  64 ragged sequences, 8 rows: 51.9 / 49.0 / 49.6 / 50.5 us with 1 / 2 / 3 / 4.
+  // With more rows a chunk itself costs more: 4 draft tokens of 48 sequences, 20 rows: 59.1 / 59.8 / 62.1 with 1 / 2 / 3.
+  // Where an SM has two blocks, a chunk is half as long: 128 sequences in 8 bits, 8 rows: 72.8 / 66.4 / 67.6 / 70.4 with 2 /
+  // 3 / 4 / 5.
   p.lead = (p.rows <= 16 ? 2 : 1) + blocks_per_sm(c->dtype == XCB_DTYPE_E4M3, dim_class(p.dim), wm) - 1;
   p.group_div = fast_div((uint32_t)p.group);
   p.head_div = fast_div((uint32_t)p.row_tiles);

@@ -382,7 +382,8 @@ class PagedKVCache:
         ``q`` [B, L, q_heads, D] (or [B, q_heads, D]: one token each): the last L tokens of sequences ``seqs`` (int32
         [B], default 0 .. B-1), already stored.  Each sees itself and what comes before it, with ``window`` the last
         ``window`` positions only.  ``scale`` defaults to D^-0.5.  Returns ``out`` like q, and with ``return_lse`` the
-        natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf."""
+        natural log-sum-exp fp32 [B, L, q_heads]; a token that sees nothing gets zeros and -inf.  L is at most 65536, and
+        L * q_heads / kv_heads 2^20."""
         layer, window = index(layer), min(index(window), 0x7fffffff)  # no sequence is longer
         if scale is not None:
             scale = float(scale)
