@@ -141,3 +141,19 @@ def test_a_window_longer_than_any_sequence(cuda_device, window):
     want, wlse = cache.attend(0, q, return_lse=True)
     assert torch.equal(out, want) and torch.equal(lse, wlse)
     assert not out[:, :6].any() and (lse[:, :6] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+def test_values_that_are_all_infinite(cuda_device, dt):
+    """Every output is looked up, in whole and in split sequences, and one of another sign anywhere makes it NaN."""
+    n, group = 5000, 6
+    kv = torch.randn((2, 2, n, 96), generator=torch.Generator().manual_seed(1)).to(dt)
+    kv[1] = -math.inf
+    kv[1, 1, 4321, 95] = math.inf
+    q = torch.randn((40, 2, 2 * group, 96), generator=torch.Generator().manual_seed(2)).to(dt).to(cuda_device)
+    cache = one_text(cuda_device, kv, 40)
+    for rows in (40, 2):
+        out = cache.attend(0, q[:rows])
+        assert (out[:, :, :group] == -math.inf).all() and (out[:, :, group:, :95] == -math.inf).all()
+        assert torch.isnan(out[:, :, group:, 95]).all()
+    assert cache.check_device_status() == 0

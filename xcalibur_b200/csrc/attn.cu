@@ -25,7 +25,7 @@
 // Measured, 8 query heads a kv head of 128: one sequence of 131072 tokens 51 us (80% of a copy's rate; 55 us on one GPU of
 // four), 64 of up to 8192 tokens 49 us (81%), 777 tokens 8.5 us (latency: plan, first stage, join kernel); 8 bits, 128
 // sequences 66 us (58%: each value is converted to 16 bits before its tensor step; f16 queries 73.5 us, whose probabilities
-// go in two parts); 4 draft tokens of 48 sequences, 20 rows 59 us (45%: 12 of 32 rows of a tile are empty, and
+// go in two parts); 4 draft tokens of 48 sequences, 20 rows 58 us (45%: 12 of 32 rows of a tile are empty, and
 // probabilities go in two parts).  A prompt of 4096 tokens, 4 kv heads, bf16: 3.1 ms, 3% of the dense products' rate for
 // what it has to compute, and no less under a window: tiles compute hidden positions too.
 //
@@ -792,48 +792,62 @@ __global__ void __launch_bounds__(Shape<DP, F8, WM>::kThreads, Shape<DP, F8, WM>
 
 // Puts what they should be in the place of the marks in a segment's outputs (a warp a row, W dimensions a lane, as the
 // join): weights are positive, so infinite values of one sign are the result, values of both signs or a NaN among them
-// make it NaN.  One lane reads the columns of its dimensions: a path for values that are broken already.
+// make it NaN.  The warp reads the columns of one lane's dimensions at a time, 128 positions a round: a path for values that
+// are broken already (one infinite value under 131072 tokens: 3.8 ms instead of 0.05).
 template <typename T, int W>
 __device__ __noinline__ void mend(const AttnParams& p, int rt, int b, int j) {
-  const int h = fdiv(j, p.head_div), tile0 = (j - h * p.row_tiles) * rt, d = (threadIdx.x & 31) * W;
+  const int h = fdiv(j, p.head_div), tile0 = (j - h * p.row_tiles) * rt, lane = threadIdx.x & 31;
   int seq, first;
   const int len = visible(p, b, &seq, &first);
-  if (d >= p.dim) return;
   for (int r = tile0 + blockIdx.y * 8 + (threadIdx.x >> 5); r < min(tile0 + rt, p.rows); r += gridDim.y * 8) {
     const int tok = fdiv(r, p.group_div);
     const int64_t place = ((int64_t)b * p.new_tokens + tok) * p.q_heads + h * p.group + r - tok * p.group;
-    uint16_t* const out = (uint16_t*)p.out + place * p.dim + d;
-    uint32_t want = 0, up = 0, down = 0, nan = 0;  // a bit a dimension
-#pragma unroll
-    for (int w = 0; w < W; ++w) want |= (uint32_t)(out[w] == kMark) << w;
-    if (!want) continue;
-    const int end = len - p.new_tokens + tok + 1;
-    for (int pos = p.window && end > p.window ? end - p.window : 0; pos < end && ((nan | (up & down)) & want) != want; ++pos) {
-      const int pi = fdiv(pos, p.kv.page_div);
-      const int page = p.kv.table[(int64_t)seq * p.kv.max_pages + pi];
-      if (page < 0 || page >= p.kv.num_pages) continue;
-      const int64_t at = ((int64_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size);
-      const uint16_t* const v = reinterpret_cast<const uint16_t*>(p.kv.k + p.kv.plane) + at * p.dim + d;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const uint32_t x = v[w];
-        if ((x & 0x7fffu) < kInf<T>) continue;
-        ((x & 0x7fffu) > kInf<T> ? nan : x >> 15 ? down : up) |= 1u << w;
-      }
-    }
+    uint16_t* const out = (uint16_t*)p.out + place * p.dim;
+    uint32_t mine = 0;  // a bit a dimension
 #pragma unroll
     for (int w = 0; w < W; ++w)
-      if (want >> w & 1) out[w] = (~nan & (up ^ down)) >> w & 1 ? (uint16_t)(kInf<T> | (down >> w & 1) << 15) : 0x7fff;
+      if (lane * W < p.dim && out[lane * W + w] == kMark) mine |= 1u << w;
+    const int end = len - p.new_tokens + tok + 1, from = p.window && end > p.window ? end - p.window : 0;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, mine != 0); todo; todo &= todo - 1) {
+      const int who = __ffs(todo) - 1;
+      const uint32_t want = __shfl_sync(0xffffffffu, mine, who);
+      uint32_t seen = 0;  // +inf, -inf and NaN, 8 bits each
+      for (int pos0 = from; pos0 < end; pos0 += 128) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int pos = pos0 + u * 32 + lane;
+          if (pos >= end) continue;
+          const int pi = fdiv(pos, p.kv.page_div);
+          const int page = p.kv.table[(int64_t)seq * p.kv.max_pages + pi];
+          if (page < 0 || page >= p.kv.num_pages) continue;
+          const int64_t at = ((int64_t)page * p.kv.kv_heads + h) * p.kv.page_size + (pos - pi * p.kv.page_size);
+          const uint16_t* const v = reinterpret_cast<const uint16_t*>(p.kv.k + p.kv.plane) + at * p.dim + who * W;
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const uint32_t x = v[w], size = x & 0x7fffu;
+            if (size >= kInf<T>) seen |= 1u << (w + (size > kInf<T> ? 16 : x >> 15 ? 8 : 0));
+          }
+        }
+        seen = __reduce_or_sync(0xffffffffu, seen);
+        if (((seen >> 16 | (seen & seen >> 8)) & want) == want) break;
+      }
+      if (lane != who) continue;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t up = seen >> w & 1, down = seen >> (w + 8) & 1, nan = seen >> (w + 16) & 1;
+        if (want >> w & 1) out[lane * W + w] = !nan && up != down ? (uint16_t)(kInf<T> | down << 15) : 0x7fff;
+      }
+    }
   }
 }
 
 // Joins the parts of the split segment that block blockIdx.x of attn_kernel began, if it did: a warp takes a row at a
 // time, a lane DP / 32 dimensions, parts in run order.  And mends the outputs that the block marked.  Bound: latency, two
-// or three rounds of reads.  Two blocks an SM: with the registers that one takes when free, 444 blocks of a call run in
-// three rounds (verification 61.7 us instead of 59.1); three an SM spill (63.3).
+// or a few rounds of reads.  Two blocks an SM, of which a call has up to 2368: as many parts are read at once as that leaves
+// registers for (verification 58.4 us; with 64 values a lane it spills, 59.9, or has one block an SM, 61.7).
 template <typename T, bool F8, int DP>
 __global__ void __launch_bounds__(256, 2) join_kernel(const __grid_constant__ AttnParams p, int rt) {
-  constexpr int W = DP / 32, U = 64 / W;  // parts whose rows are read at once
+  constexpr int W = DP / 32, U = W == 8 ? 4 : 8;  // parts whose rows are read at once
   pdl_wait();
   const int4 sp = p.splits[blockIdx.x];
   if constexpr (!F8) {
@@ -916,7 +930,7 @@ __global__ void __launch_bounds__(256, 2) join_kernel(const __grid_constant__ At
     }
     if (p.lse && lane == 0) p.lse[at] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
   }
-  if (odd) mend<T, W>(p, rt, sp.x, sp.y);
+  if (__any_sync(0xffffffffu, odd)) mend<T, W>(p, rt, sp.x, sp.y);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
