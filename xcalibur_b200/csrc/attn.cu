@@ -24,7 +24,7 @@
 //
 // Measured, 8 query heads a kv head of 128: one sequence of 131072 tokens 51 us (80% of a copy's rate; 55 us on one GPU of
 // four), 64 of up to 8192 tokens 49 us (81%), 777 tokens 8.5 us (latency: plan, first stage, join kernel); 8 bits, 128
-// sequences 66 us (58%: each value is converted to 16 bits before its tensor step; f16 queries 73.5 us, whose probabilities
+// sequences 66 us (59%: each value is converted to 16 bits before its tensor step; f16 queries 72.5 us, whose probabilities
 // go in two parts); 4 draft tokens of 48 sequences, 20 rows 58 us (45%: 12 of 32 rows of a tile are empty, and
 // probabilities go in two parts).  A prompt of 4096 tokens, 4 kv heads, bf16: 3.1 ms, 3% of the dense products' rate for
 // what it has to compute, and no less under a window: tiles compute hidden positions too.

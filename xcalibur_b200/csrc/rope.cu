@@ -7,8 +7,8 @@
 // product's low 64 bits are the exact fraction of a turn; its leading 32 bits, rounded to a float's 24, give the angle
 // within 2^-26 turns (1e-7 radians) at any position.
 //
-// Bound: HBM for prompts (each value read once and written once; 8192 tokens of 40 heads of 128 move 168 MB in 33.4 us,
-// 77% of a copy's rate; 48.7 us into 8 bits, 50%: two divisions a pair of values), latency for a decode step (one token
+// Bound: HBM for prompts (each value read once and written once; 8192 tokens of 40 heads of 128 move 168 MB in 33.5 us,
+// 76% of a copy's rate; 48.3 us into 8 bits, 50%: two divisions a pair of values), latency for a decode step (one token
 // 3.7 us, 64 tokens into 8 bits 4.8 us: a round of loads, the page lookup and the stores).  A head is held by D / 8
 // lanes, 16 bytes each, so the norm is a few shuffles.  The sines of a token are computed once per block and shared
 // through shared memory.
