@@ -69,7 +69,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         split = src == "attn.cu"
         done = subprocess.run(cmd + (["-Xptxas", "-v"] if split else []), stderr=subprocess.PIPE if split else None, text=True)
         if split:
-            sys.stderr.writelines(line for line in done.stderr.splitlines(True) if not line.startswith(("ptxas info", "    ")))
+            sys.stderr.writelines(line for line in done.stderr.splitlines(True)  # the report stays out, if all is well
+                                  if done.returncode or not line.startswith(("ptxas info", "    ")))
         done.check_returncode()
         if split:
             check_register_split(done.stderr)
